@@ -6,7 +6,7 @@ set -e
 cd "$(dirname "$0")/../unet_amd/csrc"
 name=$1; src=$2; shift 2
 D=${UNETK_AB_DIR:-build_ab}; mkdir -p ../../$D
-hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result "$@" -c "$src" -o ../../$D/${name}_${src%.hip}.o
+hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c "$src" -o ../../$D/${name}_${src%.hip}.o
 objs=""
 for o in *.o; do [ "$o" = "${src%.hip}.o" ] || objs="$objs $o"; done
 hipcc --offload-arch=gfx950 -shared -fPIC -o ../../$D/libunetk_${name}.so $objs ../../$D/${name}_${src%.hip}.o
