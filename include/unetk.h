@@ -407,6 +407,48 @@ int unetk_window_attn_any_bwd(const void* qkv, const void* dout, void* dqkv, con
  * max_heads = the largest head count among them.  Same bits as the in-place sum. */
 int unetk_dtable_reduce_batched(const int64_t* jobs, int njobs, int max_heads, unetk_stream_t stream);
 
+/* ---- norms around a token branch, fused with its gate, DropPath factor and residual ------
+ * h = post(f), or f where post_w is null;  r = res_scale * x + keep[row / rows_per_sample] * gate * h;
+ * n = pre(r) where pre_w is not null.  rms == 0: LayerNorm ((v - mean) * rstd * w + b), else RMSNorm (v * rms * w + b);
+ * eps goes under the root.  x, f (and dr, dn): M rows of C elements of `dtype`, the rows ldx, ldf (lddr, lddn) elements
+ * apart; r, n, dx, df dense.  gate, post_w, post_b, pre_w, pre_b: C floats, each may be null (post_b / pre_b only with
+ * the weight); keep: one float a sample, or null.  stats (nullable in the forward pass): [M][4] floats, mean and rstd of
+ * f and of r, 16-byte aligned.  n is taken from the unrounded r.  C is at most unetk_gated_norm_max_channels(). */
+int unetk_gated_norm_max_channels(void);
+int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
+                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                         const float* pre_w, const float* pre_b, int rms, float eps, void* r, void* n, float* stats,
+                         int64_t M, int C, int dtype, unetk_stream_t stream);
+/* The gradients, from dr (of r; may be null when dn is not) and dn (of n; given exactly when pre_w is): dx, df, and
+ * the parameters' (C floats each, null: not wanted; those of a parameter that is null have to be null).  stats: what
+ * the forward pass left.  partials: unetk_gated_norm_bwd_rows(M, C) * 5 * C floats of scratch.  No atomics: the
+ * same bits every time. */
+int unetk_gated_norm_bwd_rows(int64_t M, int C);
+int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t lddn, const void* x, int64_t ldx,
+                         const void* f, int64_t ldf, const float* stats, const float* gate, const float* keep,
+                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                         const float* pre_w, int rms, void* dx, void* df, float* dgate, float* dpost_w, float* dpost_b,
+                         float* dpre_w, float* dpre_b, float* partials, int64_t M, int C, int dtype,
+                         unetk_stream_t stream);
+
+/* ---- microscaled 4-bit floating point (OCP MX, MXFP4) -----------------------------------
+ * A (rows, K) matrix in blocks of 32 along K: E2M1 elements and one E8M0 scale 2^se a block, se = floor(log2 max|x|) - 2
+ * (not below -127), elements x / 2^se rounded half to even and held to 6.  A block with a NaN or an infinity is NaN as a whole.
+ * codes and scales (unetk_mx_codes_bytes / unetk_mx_scales_bytes, 16-byte aligned) are in the order in which the matrix
+ * instruction reads them, the same for activations and weights. */
+int64_t unetk_mx_codes_bytes(int64_t rows, int64_t K);
+int64_t unetk_mx_scales_bytes(int64_t rows, int64_t K);
+int unetk_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int dtype, void* codes, void* scales,
+                      unetk_stream_t stream);
+int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int64_t ldo, int dtype,
+                        unetk_stream_t stream);
+/* out[m][n] = act(sum_k x[m][k] * w[n][k] + bias[n]) + resid[m][n], both operands quantised: x (M, K), w (N, K).
+ * bias: N floats or null; act: 0 none, 1 ReLU, 2 GELU (erf form); resid: rows of N elements of `dtype`, ldr apart, or
+ * null; out: rows ldo apart.  Sums in fp32. */
+int unetk_mx_linear(const void* xcodes, const void* xscales, const void* wcodes, const void* wscales, void* out, int64_t ldo,
+                    int64_t M, int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
+                    unetk_stream_t stream);
+
 /* ---- optimizer tail: clip_grad_norm_ + AdamW over a list of fp32 tensors ----------------
  * enhanced_training_multi_loss.py:758-763 (AdamW), :827-829 (clip_grad_norm_(1.0), step);
  * swin_unet_model.py:836-842.  Tensors are given as device arrays of pointers + sizes; `chunks`

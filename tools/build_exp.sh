@@ -5,7 +5,7 @@ set -e
 cd "$(dirname "$0")/../unet_amd/csrc"
 name=$1; src=$2; shift 2
 mkdir -p ../../exp_ab
-hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result "$@" -c "$src" -o ../../exp_ab/${name}_${src%.hip}.o
+hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c "$src" -o ../../exp_ab/${name}_${src%.hip}.o
 objs=""
 for o in *.o; do [ "$o" = "${src%.hip}.o" ] || objs="$objs $o"; done
 hipcc --offload-arch=gfx950 -shared -fPIC -o ../../exp_ab/libunetk_${name}.so $objs ../../exp_ab/${name}_${src%.hip}.o

@@ -7,7 +7,7 @@ src = sys.argv[1]
 flt = sys.argv[2] if len(sys.argv) > 2 else ""
 extra = sys.argv[3:]
 csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "unet_amd", "csrc")
-cmd = ["hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wno-unused-result", "-c", src, "-o",
+cmd = ["hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", src, "-o",
        "/tmp/kernel_regs.o", "-Rpass-analysis=kernel-resource-usage"] + extra
 out = subprocess.run(cmd, cwd=csrc, capture_output=True, text=True).stderr
 rows, cur = [], None

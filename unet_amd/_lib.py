@@ -121,6 +121,15 @@ _SIGNATURES = {
     "unetk_window_attn_fwd": (I, [P, P, P, I, I, I, I, I, I, I, F, I, P]),
     "unetk_window_attn_bwd": (I, [P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P]),
     "unetk_dtable_reduce_batched": (I, [P, I, I, P]),
+    "unetk_gated_norm_max_channels": (I, []),
+    "unetk_gated_norm_fwd": (I, [P, L, P, L, P, P, L, F, P, P, P, P, I, F, P, P, P, L, I, I, P]),
+    "unetk_gated_norm_bwd_rows": (I, [L, I]),
+    "unetk_gated_norm_bwd": (I, [P, L, P, L, P, L, P, L, P, P, P, L, F, P, P, P, I, P, P, P, P, P, P, P, P, L, I, I, P]),
+    "unetk_mx_codes_bytes": (L, [L, L]),
+    "unetk_mx_scales_bytes": (L, [L, L]),
+    "unetk_mx_quantize": (I, [P, L, L, L, I, P, P, P]),
+    "unetk_mx_dequantize": (I, [P, P, L, L, P, L, I, P]),
+    "unetk_mx_linear": (I, [P, P, P, P, P, L, L, L, L, P, I, P, L, I, P]),
     "unetk_window_attn_any_supported": (I, [I, I]),
     "unetk_window_attn_any_fwd": (I, [P, P, P, I, I, I, I, I, I, I, I, F, I, P]),
     "unetk_window_attn_any_bwd": (I, [P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P]),

@@ -1,0 +1,445 @@
+// Norm behind a branch, gate, residual and norm in front of the next branch, in one pass each way (gfx950).
+//
+//   h = post(f) (or f)      r = res_scale * x + keep[sample] * gate * h      n = pre(r)
+//
+// post and pre are LayerNorm ((v - mean) * rstd * w + b) or RMSNorm (v * rms * w + b) over the C channels of a row;
+// f is the branch's output, x the residual stream, keep the DropPath factor of the row's sample, gate one factor a
+// channel.  Backward, from dr (the residual stream's gradient) and dn:
+//   rhat = (r - mean) rstd, q = dn w_pre:   g = dr + rstd (q - mean(q) - rhat mean(q rhat)),  dx = res_scale g
+//   u = keep g:  dgate = sum u h, dh = u gate;   fhat = (f - mean) rstd, p = dh w_post:
+//   df = rstd (p - mean(p) - fhat mean(p fhat));  dw_pre = sum dn rhat, db_pre = sum dn, dw_post = sum dh fhat, db_post = sum dh
+// (RMSNorm: no means of v, q and p.)  HBM-bound: the forward pass moves 4 tensors, the backward pass 6, a few dozen
+// operations an element.  All arithmetic is fp32; r, n, dx, df are rounded once, when they are stored.  n comes from the
+// unrounded r (which is in registers), and the backward pass forms r again from x and f for the same reason: it reads
+// as many bytes as with a stored r.
+#include "common.h"
+
+namespace {
+
+struct NormArgs {
+  const void* x;
+  const void* f;
+  const void* dr;
+  const void* dn;
+  int64_t ldx, ldf, lddr, lddn;
+  const float *gate, *keep, *post_w, *post_b, *pre_w, *pre_b;
+  const float* stats_in;
+  float* stats_out;      // [M][4]: mean and rstd of f, mean and rstd of r
+  void* o0;              // r / dx
+  void* o1;              // n / df
+  float* partials;       // [workgroups][5][C]
+  uint32_t M, rps;       // rows; rows per sample
+  int C, rms;
+  float res_scale, eps;
+};
+
+// The elements of a row that one of its G lanes holds: N = NV 16-byte vectors.  Whole vectors where rows are 16-byte
+// aligned (VEC), else single elements with neighbouring lanes on neighbouring channels.
+template <typename T, int G, int NV, bool VEC> struct Lane {
+  static constexpr int E = Vec16<T>::N, N = NV * E;
+  int gl, C;
+  __device__ __forceinline__ int chan(int i) const { return VEC ? ((i / E) * G + gl) * E + i % E : i * G + gl; }
+  __device__ __forceinline__ bool has(int i) const { return (VEC ? ((i / E) * G + gl) * E : i * G + gl) < C; }
+  struct Raw {
+    Vec16<T> v[NV];
+  };
+  __device__ __forceinline__ void load(Raw& r, const T* row) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      r.v[k] = zero16<T>();
+      if (VEC) {
+        if (has(k * E)) r.v[k] = load16(row + chan(k * E));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (has(k * E + e)) r.v[k].v[e] = row[chan(k * E + e)];
+      }
+    }
+  }
+  static __device__ __forceinline__ float at(const Raw& r, int i) { return to_f32(r.v[i / E].v[i % E]); }
+  __device__ __forceinline__ void store(T* row, const float (&d)[N]) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (VEC) {
+        Vec16<T> o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(d[k * E + e]);
+        if (has(k * E)) store16(row + chan(k * E), o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (has(k * E + e)) row[chan(k * E + e)] = from_f32<T>(d[k * E + e]);
+      }
+    }
+  }
+  __device__ __forceinline__ void param(float (&d)[N], const float* p, float none) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = (p != nullptr && has(i)) ? p[chan(i)] : none;
+  }
+};
+
+constexpr int threads_of(int G) { return G > 256 ? G : 256; }
+
+// Sums over the G lanes of a row.  Rows of more than a wave go through LDS (two areas in turn: the barrier of the next
+// call is what frees this one's).
+template <int G> struct RowSum {
+  float (*red)[2][threads_of(G) / 64];
+  int phase = 0;
+  __device__ __forceinline__ void sum2(float& a, float& b) {
+    constexpr int W = G < 64 ? G : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+      a += __shfl_xor(a, o, 64);
+      b += __shfl_xor(b, o, 64);
+    }
+    if (G > 64) {
+      constexpr int WPR = G / 64;
+      const int wave = threadIdx.x >> 6, w0 = wave / WPR * WPR;
+      if ((threadIdx.x & 63) == 0) {
+        red[phase][0][wave] = a;
+        red[phase][1][wave] = b;
+      }
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        a += red[phase][0][w0 + w];
+        b += red[phase][1][w0 + w];
+      }
+      phase ^= 1;
+    }
+  }
+  __device__ __forceinline__ float sum(float a) {
+    float b = 0.f;
+    sum2(a, b);
+    return a;
+  }
+};
+
+// mean (0 for RMSNorm) and 1 / sqrt(mean square distance from it + eps) of the row whose elements the lanes hold: from
+// registers, in two passes, so that rows far from zero keep their digits
+template <typename L, int G>
+__device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], RowSum<G>& rs, const NormArgs& a, float inv_c,
+                                        float& mean, float& rstd) {
+  mean = 0.f;
+  if (!a.rms) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < L::N; ++i) s += v[i];
+    mean = rs.sum(s) * inv_c;
+  }
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < L::N; ++i) {
+    const float d = ln.has(i) ? v[i] - mean : 0.f;
+    q += d * d;
+  }
+  rstd = 1.0f / sqrtf(rs.sum(q) * inv_c + a.eps);
+}
+
+template <typename T, int G, int NV, bool VEC>
+__global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs a) {
+  using L = Lane<T, G, NV, VEC>;
+  constexpr int N = L::N, RPB = threads_of(G) / G;
+  __shared__ float red[2][2][threads_of(G) / 64];
+  RowSum<G> rs{red};
+  const L ln{(int)(threadIdx.x % G), a.C};
+  const uint32_t rg = threadIdx.x / G;
+  const float inv_c = 1.0f / (float)a.C;
+  const bool post = a.post_w != nullptr, pre = a.pre_w != nullptr;
+  float gate[N], qw[N], qb[N], pw[N], pb[N];
+  ln.param(gate, a.gate, 1.f);
+  ln.param(qw, a.post_w, 1.f);
+  ln.param(qb, a.post_b, 0.f);
+  ln.param(pw, a.pre_w, 1.f);
+  ln.param(pb, a.pre_b, 0.f);
+  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += gridDim.x * RPB) {      // (the same trips for every wave)
+    const bool live = row0 + rg < a.M;
+    const uint32_t row = live ? row0 + rg : row0;
+    typename L::Raw xr, fr;
+    ln.load(xr, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
+    ln.load(fr, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
+    const float keep = a.keep != nullptr ? a.keep[row / a.rps] : 1.f;
+    float h[N], r[N];
+    float fm = 0.f, fs = 0.f, rm = 0.f, rsd = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = L::at(fr, i);
+    if (post) {
+      moments(ln, h, rs, a, inv_c, fm, fs);
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] = (h[i] - fm) * fs * qw[i] + qb[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = ln.has(i) ? L::at(xr, i) * a.res_scale + keep * (gate[i] * h[i]) : 0.f;
+    if (live) ln.store(reinterpret_cast<T*>(a.o0) + (int64_t)row * a.C, r);
+    if (pre) {
+      moments(ln, r, rs, a, inv_c, rm, rsd);
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[i] = (r[i] - rm) * rsd * pw[i] + pb[i];
+      if (live) ln.store(reinterpret_cast<T*>(a.o1) + (int64_t)row * a.C, r);
+    }
+    if (a.stats_out != nullptr && live && ln.gl == 0)
+      *reinterpret_cast<f32x4*>(a.stats_out + 4 * (int64_t)row) = f32x4{fm, fs, rm, rsd};
+  }
+}
+
+// Each workgroup walks rows blockIdx.x * RPB, + gridDim.x * RPB, ... and keeps its share of the five parameter
+// gradients in registers; they leave as one [5][C] row of partials a workgroup, added in a fixed order by
+// column_sums_kernel: no atomics, the same bits every time.
+template <typename T, int G, int NV, bool VEC>
+__global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs a) {
+  using L = Lane<T, G, NV, VEC>;
+  constexpr int N = L::N, RPB = threads_of(G) / G;
+  __shared__ float red[2][2][threads_of(G) / 64];
+  __shared__ float xch[RPB > 1 ? threads_of(G) * N : 1];
+  RowSum<G> rs{red};
+  const L ln{(int)(threadIdx.x % G), a.C};
+  const uint32_t rg = threadIdx.x / G;
+  const float inv_c = 1.0f / (float)a.C;
+  const bool post = a.post_w != nullptr, pre = a.pre_w != nullptr;
+  float gate[N], qw[N], qb[N], pw[N], acc[5][N];
+  ln.param(gate, a.gate, 1.f);
+  ln.param(qw, a.post_w, 1.f);
+  ln.param(qb, a.post_b, 0.f);
+  ln.param(pw, a.pre_w, 0.f);
+#pragma unroll
+  for (int s = 0; s < 5; ++s)
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[s][i] = 0.f;
+  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += gridDim.x * RPB) {
+    const bool live = row0 + rg < a.M;
+    const uint32_t row = live ? row0 + rg : row0;
+    typename L::Raw xr, fr, dr, dn;
+    ln.load(fr, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
+    if (pre) {
+      ln.load(xr, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
+      ln.load(dn, reinterpret_cast<const T*>(a.dn) + (int64_t)row * a.lddn);
+    }
+    if (a.dr != nullptr) {
+      ln.load(dr, reinterpret_cast<const T*>(a.dr) + (int64_t)row * a.lddr);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) dr.v[k] = zero16<T>();
+    }
+    const float keep = a.keep != nullptr ? a.keep[row / a.rps] : 1.f;
+    const f32x4 st = *reinterpret_cast<const f32x4*>(a.stats_in + 4 * (int64_t)row);
+    float g[N], h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      h[i] = L::at(fr, i);
+      g[i] = L::at(dr, i);
+    }
+    if (post) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] = (h[i] - st[0]) * st[1] * qw[i] + qb[i];
+    }
+    if (pre) {
+      float s1 = 0.f, s2 = 0.f, rhat[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float r = L::at(xr, i) * a.res_scale + keep * (gate[i] * h[i]);
+        rhat[i] = ln.has(i) ? (r - st[2]) * st[3] : 0.f;
+        const float d = live ? L::at(dn, i) : 0.f, q = d * pw[i];
+        acc[0][i] += d * rhat[i];
+        acc[1][i] += d;
+        s1 += q;
+        s2 += q * rhat[i];
+      }
+      rs.sum2(s1, s2);
+      s1 = a.rms ? 0.f : s1 * inv_c;
+      s2 *= inv_c;
+#pragma unroll
+      for (int i = 0; i < N; ++i) g[i] += st[3] * (L::at(dn, i) * pw[i] - s1 - rhat[i] * s2);
+    }
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = a.res_scale * g[i];
+    if (live) ln.store(reinterpret_cast<T*>(a.o0) + (int64_t)row * a.C, o);
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f;
+      acc[2][i] += u * h[i];
+      o[i] = u * gate[i];
+      if (post) {
+        const float fh = (L::at(fr, i) - st[0]) * st[1];
+        acc[3][i] += o[i] * fh;
+        acc[4][i] += o[i];
+        o[i] *= qw[i];
+        s1 += o[i];
+        s2 += o[i] * fh;
+      }
+    }
+    if (post) {
+      rs.sum2(s1, s2);
+      s1 = a.rms ? 0.f : s1 * inv_c;
+      s2 *= inv_c;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = st[1] * (o[i] - s1 - (L::at(fr, i) - st[0]) * st[1] * s2);
+    }
+    if (live) ln.store(reinterpret_cast<T*>(a.o1) + (int64_t)row * a.C, o);
+  }
+  float* out = a.partials + (int64_t)blockIdx.x * 5 * a.C;
+#pragma unroll
+  for (int s = 0; s < 5; ++s) {
+    if (s < 2 ? !pre : (s == 2 ? a.gate == nullptr : !post)) continue;      // (uniform)
+    if (RPB == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (ln.has(i)) out[s * a.C + ln.chan(i)] = acc[s][i];
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) xch[(rg * N + i) * G + ln.gl] = acc[s][i];
+      __syncthreads();
+      for (int j = threadIdx.x; j < N * G; j += threads_of(G)) {
+        const L lj{j % G, a.C};
+        const int i = j / G;
+        float t = 0.f;
+        for (int w = 0; w < RPB; ++w) t += xch[w * N * G + j];
+        if (lj.has(i)) out[s * a.C + lj.chan(i)] = t;
+      }
+    }
+  }
+}
+
+// out[s][c] = sum over the rows of partials [rows][5][C], 64 columns of one of the five a workgroup
+struct SumOuts {
+  float* p[5];
+};
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ partials, int rows, int C, SumOuts o) {
+  __shared__ double red[16][64];
+  const int s = blockIdx.y, col = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
+  if (o.p[s] == nullptr) return;
+  double t = 0.0;
+  if (col < C)
+    for (int r = rl; r < rows; r += 16) t += (double)partials[((int64_t)r * 5 + s) * C + col];
+  red[rl][threadIdx.x & 63] = t;
+  __syncthreads();
+  if (rl == 0 && col < C) {
+    for (int w = 1; w < 16; ++w) t += red[w][threadIdx.x];
+    o.p[s][col] = (float)t;
+  }
+}
+
+constexpr int NORM_MAX_C = 8192;
+
+// lanes a row and 8-element groups a lane: the fewest lanes that hold the row in eight elements each, from four lanes
+// up to eight waves
+struct Shape {
+  int G, K;
+};
+Shape norm_shape(int C) {
+  const int need = (C + 7) / 8;
+  int G = 4;
+  while (G < need && G < 512) G *= 2;
+  return {G, (need + G - 1) / G > 1 ? 2 : 1};
+}
+
+unsigned norm_grid(int64_t M, int C, int cap) {
+  const int rpb = threads_of(norm_shape(C).G) / norm_shape(C).G;
+  const int64_t b = (M + rpb - 1) / rpb;
+  return (unsigned)(b < cap ? b : cap);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+#define NORM_LAUNCH(KERNEL, T, G_, K_, VEC_)                                                                  \
+  hipLaunchKernelGGL((KERNEL<T, G_, K_ * (8 / Vec16<T>::N), VEC_>), dim3(grid), dim3(threads_of(G_)), 0, stream, a)
+#define NORM_VEC(KERNEL, T, G_, K_)              \
+  do {                                           \
+    if (vec) NORM_LAUNCH(KERNEL, T, G_, K_, true); \
+    else NORM_LAUNCH(KERNEL, T, G_, K_, false);  \
+  } while (0)
+#define NORM_DISPATCH(KERNEL, T)                                   \
+  do {                                                             \
+    const Shape sh = norm_shape(a.C);                              \
+    switch (sh.G) {                                                \
+      case 4: NORM_VEC(KERNEL, T, 4, 1); break;                    \
+      case 8: NORM_VEC(KERNEL, T, 8, 1); break;                    \
+      case 16: NORM_VEC(KERNEL, T, 16, 1); break;                  \
+      case 32: NORM_VEC(KERNEL, T, 32, 1); break;                  \
+      case 64: NORM_VEC(KERNEL, T, 64, 1); break;                  \
+      case 128: NORM_VEC(KERNEL, T, 128, 1); break;                \
+      case 256: NORM_VEC(KERNEL, T, 256, 1); break;                \
+      default:                                                     \
+        if (sh.K == 1) NORM_VEC(KERNEL, T, 512, 1);                \
+        else NORM_VEC(KERNEL, T, 512, 2);                          \
+    }                                                              \
+  } while (0)
+
+int check_norm(const char* who, int64_t M, int C, int dtype, const float* keep, int64_t rps) {
+  UNETK_CHECK_ARG(dtype == UNETK_F32 || dtype == UNETK_BF16, "%s: unsupported dtype %d", who, dtype);
+  UNETK_CHECK_ARG(C >= 1 && C <= NORM_MAX_C, "%s: C=%d (1...%d)", who, C, NORM_MAX_C);
+  UNETK_CHECK_ARG(M >= 1 && M < ((int64_t)1 << 31) - (1 << 20), "%s: %lld rows", who, (long long)M);
+  UNETK_CHECK_ARG(keep == nullptr || (rps >= 1 && M % rps == 0), "%s: %lld rows are not whole samples of %lld", who,
+                  (long long)M, (long long)rps);
+  return UNETK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int unetk_gated_norm_max_channels(void) { return NORM_MAX_C; }
+
+int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
+                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                         const float* pre_w, const float* pre_b, int rms, float eps, void* r, void* n, float* stats,
+                         int64_t M, int C, int dtype, hipStream_t stream) {
+  const int rc = check_norm("gated_norm_fwd", M, C, dtype, keep, rows_per_sample);
+  if (rc != UNETK_OK) return rc;
+  UNETK_CHECK_ARG(x && f && r && ldx >= C && ldf >= C, "gated_norm_fwd: null operand or overlapping rows");
+  UNETK_CHECK_ARG((pre_w != nullptr) == (n != nullptr), "gated_norm_fwd: n goes with the norm in front");
+  UNETK_CHECK_ARG((post_w || !post_b) && (pre_w || !pre_b), "gated_norm_fwd: a norm's bias without its weight");
+  NormArgs a = {};
+  a.x = x; a.f = f; a.ldx = ldx; a.ldf = ldf; a.gate = gate; a.keep = keep; a.post_w = post_w; a.post_b = post_b;
+  a.pre_w = pre_w; a.pre_b = pre_b; a.stats_out = stats; a.o0 = r; a.o1 = n; a.M = (uint32_t)M;
+  a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms; a.res_scale = res_scale; a.eps = eps;
+  const int E = dtype == UNETK_BF16 ? 8 : 4;
+  const bool vec = C % E == 0 && ldx % E == 0 && ldf % E == 0 && aligned16(x) && aligned16(f) && aligned16(r) && aligned16(n);
+  const unsigned grid = norm_grid(M, C, 4096);
+  if (dtype == UNETK_BF16) NORM_DISPATCH(gated_norm_fwd_kernel, bf16);
+  else NORM_DISPATCH(gated_norm_fwd_kernel, float);
+  UNETK_CHECK_LAUNCH();
+  return UNETK_OK;
+}
+
+int unetk_gated_norm_bwd_rows(int64_t M, int C) {
+  return M < 1 || C < 1 || C > NORM_MAX_C ? 0 : (int)norm_grid(M, C, 1024);
+}
+
+int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t lddn, const void* x, int64_t ldx,
+                         const void* f, int64_t ldf, const float* stats, const float* gate, const float* keep,
+                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                         const float* pre_w, int rms, void* dx, void* df, float* dgate, float* dpost_w, float* dpost_b,
+                         float* dpre_w, float* dpre_b, float* partials, int64_t M, int C, int dtype, hipStream_t stream) {
+  const int rc = check_norm("gated_norm_bwd", M, C, dtype, keep, rows_per_sample);
+  if (rc != UNETK_OK) return rc;
+  UNETK_CHECK_ARG(x && f && stats && dx && df && partials && ldx >= C && ldf >= C && (dr || dn),
+                  "gated_norm_bwd: null operand or overlapping rows");
+  UNETK_CHECK_ARG((dr == nullptr || lddr >= C) && (dn == nullptr || lddn >= C), "gated_norm_bwd: overlapping rows");
+  UNETK_CHECK_ARG((pre_w != nullptr) == (dn != nullptr), "gated_norm_bwd: dn goes with the norm in front");
+  UNETK_CHECK_ARG((gate || !dgate) && (post_w || !(post_b || dpost_w || dpost_b)) && (pre_w || !(dpre_w || dpre_b)),
+                  "gated_norm_bwd: a gradient of a parameter that is not there");
+  NormArgs a = {};
+  a.x = x; a.f = f; a.dr = dr; a.dn = dn; a.ldx = ldx; a.ldf = ldf; a.lddr = lddr; a.lddn = lddn; a.gate = gate;
+  a.keep = keep; a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.stats_in = stats; a.o0 = dx; a.o1 = df;
+  a.partials = partials; a.M = (uint32_t)M; a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms;
+  a.res_scale = res_scale;
+  const int E = dtype == UNETK_BF16 ? 8 : 4;
+  const bool vec = C % E == 0 && ldx % E == 0 && ldf % E == 0 && (!dr || lddr % E == 0) && (!dn || lddn % E == 0) &&
+                   aligned16(x) && aligned16(f) && aligned16(dr) && aligned16(dn) && aligned16(dx) && aligned16(df);
+  const unsigned grid = (unsigned)unetk_gated_norm_bwd_rows(M, C);
+  if (dtype == UNETK_BF16) NORM_DISPATCH(gated_norm_bwd_kernel, bf16);
+  else NORM_DISPATCH(gated_norm_bwd_kernel, float);
+  UNETK_CHECK_LAUNCH();
+  if (dgate || dpost_w || dpost_b || dpre_w || dpre_b) {
+    const SumOuts o = {{dpre_w, dpre_b, dgate, dpost_w, dpost_b}};
+    hipLaunchKernelGGL(column_sums_kernel, dim3(cdiv(C, 64), 5), dim3(1024), 0, stream, partials, (int)grid, C, o);
+    UNETK_CHECK_LAUNCH();
+  }
+  return UNETK_OK;
+}
+
+}  // extern "C"

@@ -4,7 +4,7 @@ Activations are NHWC tensors of the compute dtype (float32 or bfloat16) living o
 GPU; torch only provides their memory and the current stream.  Every function
 enqueues kernels on ``torch.cuda.current_stream()`` and returns without synchronising.
 """
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -936,3 +936,245 @@ def window_attn_bwd(qkv, dout, table, heads, shift, use_mask, defer=None, ws=8):
     if defer is not None:
         defer.add_table(partials, nblk // heads, heads, dtable)
     return dqkv, dtable
+
+
+# ------------------------------------------------------------------ norms around a branch, 4-bit products
+def _token_rows(t, what, device=None, dtype=None):
+    """(rows, row stride) of a channels-last tensor whose rows are equally spaced: a dense tensor, or a channel slice of
+    one."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    _require_cuda(t, what)
+    if t.dim() < 1:
+        raise ValueError(f"{what}: expected (..., channels), got a 0-dim tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    C = t.shape[-1]
+    rows = 1
+    for n in t.shape[:-1]:
+        rows *= n
+    if rows * C == 0 or rows == 1:
+        if C > 1 and rows == 1 and t.stride(-1) != 1:
+            raise ValueError(f"{what}: channels must be contiguous (strides {t.stride()})")
+        return rows, max(C, 1)
+    # the row axis, outermost first, sizes of one left out: each stride the next one's times its size
+    ax = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
+    ld = ax[-1][1]
+    want = ld
+    for n, st in reversed(ax):
+        if st != want:
+            raise ValueError(f"{what}: rows must be equally spaced (shape {tuple(t.shape)}, strides {t.stride()})")
+        want = st * n
+    if (C > 1 and t.stride(-1) != 1) or ld < C:
+        raise ValueError(f"{what}: channels must be contiguous and rows must not overlap (strides {t.stride()})")
+    return rows, ld
+
+
+def _vector(t, what, n, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float32 vector of {n} on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _norm_pair(p, what, C, device):
+    if p is None:
+        return None, None
+    w, b = p
+    if w is None:
+        raise ValueError(f"{what}: a norm is given by (weight, bias or None)")
+    return _vector(w, what + " weight", C, device), _vector(b, what + " bias", C, device)
+
+
+def _gated_norm_args(x, f, gate, keep, post, pre, kind):
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"gated_norm: kind {kind!r} (\"layer\" or \"rms\")")
+    M, ldx = _token_rows(x, "x")
+    dtype_code(x.dtype)
+    if not isinstance(f, torch.Tensor) or f.shape != x.shape:
+        raise ValueError(f"f: expected the shape of x, {tuple(x.shape)}")
+    _, ldf = _token_rows(f, "f", x.device, x.dtype)
+    C = x.shape[-1]
+    if not 1 <= C <= _lib.load().unetk_gated_norm_max_channels():
+        raise ValueError(f"gated_norm: {C} channels (1...{_lib.load().unetk_gated_norm_max_channels()})")
+    _vector(gate, "gate", C, x.device)
+    rps = 0
+    if keep is not None:
+        if not isinstance(keep, torch.Tensor) or keep.dim() != 1 or keep.shape[0] < 1 or M % keep.shape[0]:
+            raise ValueError(f"keep: expected one factor a sample for {M} rows")
+        _vector(keep, "keep", keep.shape[0], x.device)
+        rps = M // keep.shape[0]
+    return M, C, ldx, ldf, rps, _norm_pair(post, "post", C, x.device), _norm_pair(pre, "pre", C, x.device)
+
+
+def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=None, kind="layer", eps=1e-5, want_stats=True):
+    """The end of a token branch and the norm in front of the next one, in one pass:
+
+        h = post(f) (or f);  r = res_scale * x + keep[sample] * gate * h;  n = pre(r)
+
+    x: the residual stream, f: the branch's output, (..., C) float32 or bfloat16 with equally spaced rows (dense, or a
+    channel slice).  post, pre: (weight, bias or None) of the two norms, each may be None; kind: "layer" or "rms" (without
+    the mean).  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
+    float32.  Returns (r, n, stats): r and n dense, n None without pre; stats is what gated_norm_bwd reads (None unless
+    want_stats).  n is taken from the unrounded r."""
+    M, C, ldx, ldf, rps, (qw, qb), (pw, pb) = _gated_norm_args(x, f, gate, keep, post, pre, kind)
+    with torch.cuda.device(x.device):
+        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        n = torch.empty_like(r) if pw is not None else None
+        stats = torch.empty((M, 4), dtype=torch.float32, device=x.device) if want_stats else None
+        if M:
+            call("unetk_gated_norm_fwd", ptr(x), ldx, ptr(f), ldf, ptr(gate), ptr(keep), rps, float(res_scale), ptr(qw),
+                 ptr(qb), ptr(pw), ptr(pb), int(kind == "rms"), float(eps), ptr(r), ptr(n), ptr(stats), M, C,
+                 dtype_code(x.dtype), stream())
+    return r, n, stats
+
+
+class GatedNormGrads(NamedTuple):
+    """What gated_norm_bwd returns; a gradient of something that was not given is None."""
+    x: torch.Tensor
+    f: torch.Tensor
+    gate: Optional[torch.Tensor]
+    post_weight: Optional[torch.Tensor]
+    post_bias: Optional[torch.Tensor]
+    pre_weight: Optional[torch.Tensor]
+    pre_bias: Optional[torch.Tensor]
+
+
+def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, post=None, pre=None, kind="layer", eps=1e-5):
+    """Gradients of gated_norm_fwd (the same arguments, and its stats) from dr and dn, the gradients of r and n.  dr may
+    be None where nothing else reads r; dn is given exactly when pre is.  Sums over rows are taken in a fixed order: the
+    same bits every time."""
+    M, C, ldx, ldf, rps, (qw, qb), (pw, pb) = _gated_norm_args(x, f, gate, keep, post, pre, kind)
+    if (dn is None) != (pw is None) or (dr is None and dn is None):
+        raise ValueError("gated_norm_bwd: dn goes with pre, and one of dr and dn has to be there")
+    ld = []
+    for g, what in ((dr, "dr"), (dn, "dn")):
+        if g is not None and (not isinstance(g, torch.Tensor) or g.shape != x.shape):
+            raise ValueError(f"{what}: expected the shape of x, {tuple(x.shape)}")
+        ld.append(0 if g is None else _token_rows(g, what, x.device, x.dtype)[1])
+    if not isinstance(stats, torch.Tensor) or stats.shape != (M, 4) or stats.dtype != torch.float32 or \
+            stats.device != x.device or not stats.is_contiguous():
+        raise ValueError(f"stats: expected what gated_norm_fwd returned for these {M} rows")
+    dev = x.device
+    with torch.cuda.device(dev):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        df = torch.empty_like(dx)
+        dgate, dqw, dqb, dpw, dpb = (None if p is None else torch.empty(C, dtype=torch.float32, device=dev)
+                                     for p in (gate, qw, qb, pw, pb))
+        if M:
+            rows = _lib.load().unetk_gated_norm_bwd_rows(M, C)
+            partials = torch.empty((rows, 5, C), dtype=torch.float32, device=dev)
+            call("unetk_gated_norm_bwd", ptr(dr), ld[0], ptr(dn), ld[1], ptr(x), ldx, ptr(f), ldf, ptr(stats), ptr(gate),
+                 ptr(keep), rps, float(res_scale), ptr(qw), ptr(qb), ptr(pw), int(kind == "rms"), ptr(dx), ptr(df),
+                 ptr(dgate), ptr(dqw), ptr(dqb), ptr(dpw), ptr(dpb), ptr(partials), M, C, dtype_code(x.dtype), stream())
+        else:
+            for g in (dgate, dqw, dqb, dpw, dpb):
+                if g is not None:
+                    g.zero_()
+    return GatedNormGrads(dx, df, dgate, dqw, dqb, dpw, dpb)
+
+
+class MxTensor:
+    """A (..., K) tensor in microscaled 4-bit floating point (OCP MXFP4): blocks of 32 along K, E2M1 elements and one
+    power-of-two scale a block, in the order in which the matrix instruction reads them.  Made by mx_quantize; read by
+    mx_linear (activations or weights alike) and mx_dequantize."""
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def rows(self):
+        n = 1
+        for v in self.shape[:-1]:
+            n *= v
+        return n
+
+    def __repr__(self):
+        return f"MxTensor(shape={tuple(self.shape)}, device={self.device})"
+
+
+def mx_quantize(x) -> MxTensor:
+    """x (..., K), float32 or bfloat16 with equally spaced rows, in 4 bits: per block of 32 along K the scale
+    2^(floor(log2 max) - 2) and the elements rounded half to even to 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (larger ones:
+    6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros."""
+    rows, ld = _token_rows(x, "x")
+    code, K = dtype_code(x.dtype), x.shape[-1]
+    if K < 1:
+        raise ValueError("mx_quantize: no elements to scale (K = 0)")
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        nc = lib.unetk_mx_codes_bytes(rows, K) if rows else 0
+        if rows and not nc:
+            raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
+        codes = torch.empty(nc, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(nc // 16, dtype=torch.uint8, device=x.device)
+        if rows:
+            call("unetk_mx_quantize", ptr(x), ld, rows, K, code, ptr(codes), ptr(scales), stream())
+    return MxTensor(codes, scales, x.shape)
+
+
+def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values that q stands for, exact in float32 and in bfloat16."""
+    if not isinstance(q, MxTensor):
+        raise TypeError(f"mx_dequantize: expected an MxTensor, got {type(q).__name__}")
+    code, rows, K = dtype_code(dtype), q.rows, q.shape[-1]
+    with torch.cuda.device(q.device):
+        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        if rows:
+            call("unetk_mx_dequantize", ptr(q.codes), ptr(q.scales), rows, K, ptr(out), K, code, stream())
+    return out
+
+
+def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None):
+    """act(x @ w^T + bias) + resid with both operands in microscaled 4 bits and fp32 sums; for prediction (it has no
+    gradient).  x (..., K): a float32 or bfloat16 tensor, quantised on the way, or an MxTensor (quantised once for
+    several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none, 1 ReLU, 2 GELU (erf form);
+    resid: (..., N) of the result's type.  The result has x's type (``dtype`` for an MxTensor, bfloat16 if not given); out:
+    a (..., N) tensor or channel slice to write it to."""
+    if not isinstance(w, MxTensor) or len(w.shape) != 2:
+        raise TypeError("mx_linear: w is mx_quantize of the (N, K) weight")
+    N, K = w.shape
+    quantised = isinstance(x, MxTensor)
+    if not quantised and not isinstance(x, torch.Tensor):
+        raise TypeError(f"mx_linear: x is a tensor or an MxTensor, not {type(x).__name__}")
+    if len(x.shape) < 1 or x.shape[-1] != K:
+        raise ValueError(f"mx_linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
+    if x.device != w.device:
+        raise ValueError(f"mx_linear: x on {x.device}, w on {w.device}")
+    if act not in (0, 1, 2):
+        raise ValueError(f"mx_linear: act {act!r} (0 none, 1 ReLU, 2 GELU)")
+    if quantised:
+        dt, rows = dtype or torch.bfloat16, x.rows
+    else:
+        if dtype is not None and dtype != x.dtype:
+            raise ValueError(f"mx_linear: dtype {dtype} for x of {x.dtype}")
+        dt, rows = x.dtype, _token_rows(x, "x")[0]
+    code, shape, dev = dtype_code(dt), x.shape[:-1] + (N,), w.device
+    _vector(bias, "bias", N, dev)
+    ldo = ldr = N
+    for t, what in ((out, "out"), (resid, "resid")):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != shape):
+            raise ValueError(f"{what}: expected the shape {tuple(shape)}")
+    if out is not None:
+        ldo = _token_rows(out, "out", dev, dt)[1]
+    if resid is not None:
+        ldr = _token_rows(resid, "resid", dev, dt)[1]
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(shape, dtype=dt, device=dev)
+        if rows and N:
+            xq = x if quantised else mx_quantize(x)
+            call("unetk_mx_linear", ptr(xq.codes), ptr(xq.scales), ptr(w.codes), ptr(w.scales), ptr(out), ldo, rows, K, N,
+                 ptr(bias), act, ptr(resid), ldr, code, stream())
+    return out
