@@ -421,7 +421,7 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
                          int64_t M, int C, int dtype, unetk_stream_t stream);
 /* The gradients, from dr (of r; may be null when dn is not) and dn (of n; given exactly when pre_w is): dx, df, and
  * the parameters' (C floats each, null: not wanted; those of a parameter that is null have to be null).  stats: what
- * the forward pass left.  partials: unetk_gated_norm_bwd_rows(M, C) * 5 * C floats of scratch.  No atomics: the
+ * the forward pass left.  partials: unetk_gated_norm_bwd_rows(M, C) * 4 * C floats of scratch.  No atomics: the
  * same bits every time. */
 int unetk_gated_norm_bwd_rows(int64_t M, int C);
 int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t lddn, const void* x, int64_t ldx,

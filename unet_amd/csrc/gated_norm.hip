@@ -80,6 +80,26 @@ template <typename T, int G, int NV, bool VEC> struct Lane {
 
 constexpr int threads_of(int G) { return G > 256 ? G : 256; }
 
+// v plus its partner's: lanes 1, 2, 4 and 8 apart inside a row of 16 through DPP (the last two as mirrors: by then all
+// lanes of a half hold the same sum), 16 through the swizzle, 32 by reading the two halves' sums as scalars.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  const int i = __builtin_bit_cast(int, v);
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, true));
+}
+template <int W> __device__ __forceinline__ float lane_sum(float v) {
+  if (W >= 2) v = dpp_add<0xB1>(v);
+  if (W >= 4) v = dpp_add<0x4E>(v);
+  if (W >= 8) v = dpp_add<0x141>(v);
+  if (W >= 16) v = dpp_add<0x140>(v);
+  if (W >= 32)
+    v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));      // lane ^ 16
+  if (W >= 64) {
+    const int i = __builtin_bit_cast(int, v);
+    v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32));
+  }
+  return v;
+}
+
 // Sums over the G lanes of a row.  Rows of more than a wave go through LDS (two areas in turn: the barrier of the next
 // call is what frees this one's).
 template <int G> struct RowSum {
@@ -87,11 +107,8 @@ template <int G> struct RowSum {
   int phase = 0;
   __device__ __forceinline__ void sum2(float& a, float& b) {
     constexpr int W = G < 64 ? G : 64;
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-      a += __shfl_xor(a, o, 64);
-      b += __shfl_xor(b, o, 64);
-    }
+    a = lane_sum<W>(a);
+    b = lane_sum<W>(b);
     if (G > 64) {
       constexpr int WPR = G / 64;
       const int wave = threadIdx.x >> 6, w0 = wave / WPR * WPR;
@@ -110,6 +127,7 @@ template <int G> struct RowSum {
     }
   }
   __device__ __forceinline__ float sum(float a) {
+    if (G <= 64) return lane_sum<(G < 64 ? G : 64)>(a);
     float b = 0.f;
     sum2(a, b);
     return a;
@@ -126,7 +144,7 @@ __device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], Row
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < L::N; ++i) s += v[i];
-    mean = rs.sum(s) * inv_c;
+    mean = rs.sum(s) / (float)a.C;
   }
   float q = 0.f;
 #pragma unroll
@@ -135,6 +153,14 @@ __device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], Row
     q += d * d;
   }
   rstd = 1.0f / sqrtf(rs.sum(q) * inv_c + a.eps);
+}
+
+// One element of r, in the operations that both directions use (explicit fused multiply-adds: whatever the compiler
+// would contract in each, the backward pass finds the bits of the forward pass, and rows whose deviation is nothing but
+// rounding keep it).  gw = gate w_post, gb = gate b_post.
+__device__ __forceinline__ float norm_hat(float v, float mean, float rstd) { return (v - mean) * rstd; }
+__device__ __forceinline__ float residual(float x, float fhat, float gw, float gb, float keep, float scale) {
+  return fmaf(keep, fmaf(fhat, gw, gb), x * scale);
 }
 
 template <typename T, int G, int NV, bool VEC>
@@ -147,35 +173,47 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
   const uint32_t rg = threadIdx.x / G;
   const float inv_c = 1.0f / (float)a.C;
   const bool post = a.post_w != nullptr, pre = a.pre_w != nullptr;
-  float gate[N], qw[N], qb[N], pw[N], pb[N];
-  ln.param(gate, a.gate, 1.f);
-  ln.param(qw, a.post_w, 1.f);
-  ln.param(qb, a.post_b, 0.f);
+  // gate * (fhat * w_post + b_post) = fhat * (gate w_post) + gate b_post
+  float qw[N], qb[N], pw[N], pb[N];
+  {
+    float gate[N];
+    ln.param(gate, a.gate, 1.f);
+    ln.param(qw, a.post_w, 1.f);
+    ln.param(qb, a.post_b, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) qw[i] *= gate[i], qb[i] *= gate[i];
+  }
   ln.param(pw, a.pre_w, 1.f);
   ln.param(pb, a.pre_b, 0.f);
-  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += gridDim.x * RPB) {      // (the same trips for every wave)
+  // the next row is on its way while this one is reduced
+  typename L::Raw xn, fn;
+  auto fetch = [&](uint32_t row0) __attribute__((always_inline)) {
+    const uint32_t row = row0 + rg < a.M ? row0 + rg : a.M - 1;
+    ln.load(xn, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
+    ln.load(fn, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
+  };
+  const uint32_t step = gridDim.x * RPB;
+  if (blockIdx.x * RPB < a.M) fetch(blockIdx.x * RPB);
+  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += step) {      // (the same trips for every wave)
     const bool live = row0 + rg < a.M;
     const uint32_t row = live ? row0 + rg : row0;
-    typename L::Raw xr, fr;
-    ln.load(xr, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
-    ln.load(fr, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
+    const typename L::Raw xr = xn, fr = fn;
+    if (row0 + step < a.M) fetch(row0 + step);
     const float keep = a.keep != nullptr ? a.keep[row / a.rps] : 1.f;
     float h[N], r[N];
     float fm = 0.f, fs = 0.f, rm = 0.f, rsd = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = L::at(fr, i);
-    if (post) {
-      moments(ln, h, rs, a, inv_c, fm, fs);
+    if (post) moments(ln, h, rs, a, inv_c, fm, fs);
+    const float hs = post ? fs : 1.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) h[i] = (h[i] - fm) * fs * qw[i] + qb[i];
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) r[i] = ln.has(i) ? L::at(xr, i) * a.res_scale + keep * (gate[i] * h[i]) : 0.f;
+    for (int i = 0; i < N; ++i)
+      r[i] = ln.has(i) ? residual(L::at(xr, i), norm_hat(h[i], fm, hs), qw[i], qb[i], keep, a.res_scale) : 0.f;
     if (live) ln.store(reinterpret_cast<T*>(a.o0) + (int64_t)row * a.C, r);
     if (pre) {
       moments(ln, r, rs, a, inv_c, rm, rsd);
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[i] = (r[i] - rm) * rsd * pw[i] + pb[i];
+      for (int i = 0; i < N; ++i) r[i] = norm_hat(r[i], rm, rsd) * pw[i] + pb[i];
       if (live) ln.store(reinterpret_cast<T*>(a.o1) + (int64_t)row * a.C, r);
     }
     if (a.stats_out != nullptr && live && ln.gl == 0)
@@ -183,8 +221,10 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
   }
 }
 
-// Each workgroup walks rows blockIdx.x * RPB, + gridDim.x * RPB, ... and keeps its share of the five parameter
-// gradients in registers; they leave as one [5][C] row of partials a workgroup, added in a fixed order by
+// Each workgroup walks rows blockIdx.x * RPB, + gridDim.x * RPB, ... and keeps its share of four sums a channel in
+// registers: dn rhat, dn, u fhat and u (u = keep g; without a norm behind the branch fhat is f).  The gradients of gate,
+// w_post and b_post are these times constants of the channel: dgate = w_post sum(u fhat) + b_post sum(u), dw_post = gate
+// sum(u fhat), db_post = gate sum(u).  The sums leave as one [4][C] row of partials a workgroup, added in a fixed order by
 // column_sums_kernel: no atomics, the same bits every time.
 template <typename T, int G, int NV, bool VEC>
 __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs a) {
@@ -197,49 +237,80 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
   const uint32_t rg = threadIdx.x / G;
   const float inv_c = 1.0f / (float)a.C;
   const bool post = a.post_w != nullptr, pre = a.pre_w != nullptr;
-  float gate[N], qw[N], qb[N], pw[N], acc[5][N];
-  ln.param(gate, a.gate, 1.f);
-  ln.param(qw, a.post_w, 1.f);
-  ln.param(qb, a.post_b, 0.f);
-  ln.param(pw, a.pre_w, 0.f);
-#pragma unroll
-  for (int s = 0; s < 5; ++s)
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[s][i] = 0.f;
-  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += gridDim.x * RPB) {
-    const bool live = row0 + rg < a.M;
-    const uint32_t row = live ? row0 + rg : row0;
-    typename L::Raw xr, fr, dr, dn;
-    ln.load(fr, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
-    if (pre) {
-      ln.load(xr, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
-      ln.load(dn, reinterpret_cast<const T*>(a.dn) + (int64_t)row * a.lddn);
-    }
-    if (a.dr != nullptr) {
-      ln.load(dr, reinterpret_cast<const T*>(a.dr) + (int64_t)row * a.lddr);
-    } else {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) dr.v[k] = zero16<T>();
-    }
-    const float keep = a.keep != nullptr ? a.keep[row / a.rps] : 1.f;
-    const f32x4 st = *reinterpret_cast<const f32x4*>(a.stats_in + 4 * (int64_t)row);
-    float g[N], h[N];
+  // gate w_post, gate b_post, w_pre of this lane's channels: in registers, or, where a lane holds 16 channels and the
+  // registers do not suffice, in LDS (each lane reads back only what it wrote itself)
+  constexpr bool PL = N > 8;
+  float preg[PL ? 1 : 3][N];
+  __shared__ float plds[PL ? 3 : 1][PL ? N * G : 1];
+  auto put = [&](int s, const float (&d)[N]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      h[i] = L::at(fr, i);
-      g[i] = L::at(dr, i);
+      if (PL) plds[s][i * G + ln.gl] = d[i];
+      else preg[PL ? 0 : s][i] = d[i];
     }
-    if (post) {
+  };
+  auto prm = [&](int s, int i) __attribute__((always_inline)) { return PL ? plds[s][i * G + ln.gl] : preg[PL ? 0 : s][i]; };
+  {
+    float gate[N], w[N];
+    ln.param(gate, a.gate, 1.f);
+    ln.param(w, a.post_w, 1.f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) h[i] = (h[i] - st[0]) * st[1] * qw[i] + qb[i];
+    for (int i = 0; i < N; ++i) w[i] *= gate[i];
+    put(0, w);
+    ln.param(w, a.post_b, 0.f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] *= gate[i];
+    put(1, w);
+    ln.param(w, a.pre_w, 0.f);
+    put(2, w);
+  }
+  float acc[4][N];
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[s][i] = 0.f;
+  // the next row is on its way while this one is reduced
+  struct Next {
+    typename L::Raw x, f, dr, dn;
+    f32x4 st;
+    float keep;
+  } nx;
+  auto fetch = [&](uint32_t row0) __attribute__((always_inline)) {
+    const uint32_t row = row0 + rg < a.M ? row0 + rg : a.M - 1;
+    nx.st = *reinterpret_cast<const f32x4*>(a.stats_in + 4 * (int64_t)row);
+    nx.keep = a.keep != nullptr ? a.keep[row / a.rps] : 1.f;
+    ln.load(nx.f, reinterpret_cast<const T*>(a.f) + (int64_t)row * a.ldf);
+    if (pre) {
+      ln.load(nx.x, reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx);
+      ln.load(nx.dn, reinterpret_cast<const T*>(a.dn) + (int64_t)row * a.lddn);
     }
+    if (a.dr != nullptr) {
+      ln.load(nx.dr, reinterpret_cast<const T*>(a.dr) + (int64_t)row * a.lddr);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) nx.dr.v[k] = zero16<T>();
+    }
+  };
+  const uint32_t step = gridDim.x * RPB;
+  if (blockIdx.x * RPB < a.M) fetch(blockIdx.x * RPB);
+  for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += step) {
+    const bool live = row0 + rg < a.M;
+    const uint32_t row = live ? row0 + rg : row0;
+    const typename L::Raw xr = nx.x, fr = nx.f, dr = nx.dr, dn = nx.dn;
+    const f32x4 st = nx.st;
+    const float keep = nx.keep;
+    if (row0 + step < a.M) fetch(row0 + step);
+    const float fm = post ? st[0] : 0.f, fs = post ? st[1] : 1.f;
+    float g[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = L::at(dr, i);
     if (pre) {
       float s1 = 0.f, s2 = 0.f, rhat[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float r = L::at(xr, i) * a.res_scale + keep * (gate[i] * h[i]);
-        rhat[i] = ln.has(i) ? (r - st[2]) * st[3] : 0.f;
-        const float d = live ? L::at(dn, i) : 0.f, q = d * pw[i];
+        const float r = residual(L::at(xr, i), norm_hat(L::at(fr, i), fm, fs), prm(0, i), prm(1, i), keep, a.res_scale);
+        rhat[i] = ln.has(i) ? norm_hat(r, st[2], st[3]) : 0.f;
+        const float d = live ? L::at(dn, i) : 0.f, q = d * prm(2, i);
         acc[0][i] += d * rhat[i];
         acc[1][i] += d;
         s1 += q;
@@ -249,7 +320,7 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
       s1 = a.rms ? 0.f : s1 * inv_c;
       s2 *= inv_c;
 #pragma unroll
-      for (int i = 0; i < N; ++i) g[i] += st[3] * (L::at(dn, i) * pw[i] - s1 - rhat[i] * s2);
+      for (int i = 0; i < N; ++i) g[i] += st[3] * (L::at(dn, i) * prm(2, i) - s1 - rhat[i] * s2);
     }
     float o[N];
 #pragma unroll
@@ -258,31 +329,26 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f;
-      acc[2][i] += u * h[i];
-      o[i] = u * gate[i];
-      if (post) {
-        const float fh = (L::at(fr, i) - st[0]) * st[1];
-        acc[3][i] += o[i] * fh;
-        acc[4][i] += o[i];
-        o[i] *= qw[i];
-        s1 += o[i];
-        s2 += o[i] * fh;
-      }
+      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f, fh = norm_hat(L::at(fr, i), fm, fs);
+      acc[2][i] += u * fh;
+      acc[3][i] += u;
+      o[i] = u * prm(0, i);
+      s1 += o[i];
+      s2 += o[i] * fh;
     }
     if (post) {
       rs.sum2(s1, s2);
       s1 = a.rms ? 0.f : s1 * inv_c;
       s2 *= inv_c;
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = st[1] * (o[i] - s1 - (L::at(fr, i) - st[0]) * st[1] * s2);
+      for (int i = 0; i < N; ++i) o[i] = fs * (o[i] - s1 - norm_hat(L::at(fr, i), fm, fs) * s2);
     }
     if (live) ln.store(reinterpret_cast<T*>(a.o1) + (int64_t)row * a.C, o);
   }
-  float* out = a.partials + (int64_t)blockIdx.x * 5 * a.C;
+  float* out = a.partials + (int64_t)blockIdx.x * 4 * a.C;
 #pragma unroll
-  for (int s = 0; s < 5; ++s) {
-    if (s < 2 ? !pre : (s == 2 ? a.gate == nullptr : !post)) continue;      // (uniform)
+  for (int s = 0; s < 4; ++s) {
+    if (s < 2 && !pre) continue;      // (uniform)
     if (RPB == 1) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -303,22 +369,49 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
   }
 }
 
-// out[s][c] = sum over the rows of partials [rows][5][C], 64 columns of one of the five a workgroup
-struct SumOuts {
-  float* p[5];
+// Sums of partials [rows][4][C] down the rows, in double, and the gradients made of them: blockIdx.y 0: the norm in front
+// (d0: weight, d1: bias), 1: gate, weight and bias of the norm behind (d2, d3, d4).  16 columns a workgroup, 32 row lanes a
+// sum with eight loads in flight each (a few MB that were just written: latency, not bytes).
+struct SumArgs {
+  float *d0, *d1, *d2, *d3, *d4;
+  const float *gate, *post_w, *post_b;
 };
-__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ partials, int rows, int C, SumOuts o) {
-  __shared__ double red[16][64];
-  const int s = blockIdx.y, col = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
-  if (o.p[s] == nullptr) return;
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restrict__ partials, int rows, int C, SumArgs o) {
+  __shared__ double red[2][32][17];
+  const bool behind = blockIdx.y != 0;
+  if (behind ? !(o.d2 || o.d3 || o.d4) : !(o.d0 || o.d1)) return;
+  const int cl = threadIdx.x & 15, which = (threadIdx.x >> 4) & 1, rl = threadIdx.x >> 5, col = blockIdx.x * 16 + cl;
   double t = 0.0;
-  if (col < C)
-    for (int r = rl; r < rows; r += 16) t += (double)partials[((int64_t)r * 5 + s) * C + col];
-  red[rl][threadIdx.x & 63] = t;
+  if (col < C) {
+    const float* p = partials + (int64_t)(2 * blockIdx.y + which) * C + col;
+    for (int r0 = rl; r0 < rows; r0 += 32 * 8) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = r0 + 32 * j < rows ? p[(int64_t)(r0 + 32 * j) * 4 * C] : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t += (double)v[j];
+    }
+  }
+  red[which][rl][cl] = t;
   __syncthreads();
-  if (rl == 0 && col < C) {
-    for (int w = 1; w < 16; ++w) t += red[w][threadIdx.x];
-    o.p[s][col] = (float)t;
+  if (threadIdx.x >= 64) return;      // one wave adds: lane = (half of the row lanes, sum, column)
+  {
+    const int half = threadIdx.x >> 5;
+    t = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t += red[which][half * 16 + w][cl];
+    t += __shfl_xor(t, 32, 64);
+    const double other = __shfl_xor(t, 16, 64);
+    if (threadIdx.x >= 16 || col >= C) return;
+    if (!behind) {
+      if (o.d0) o.d0[col] = (float)t;
+      if (o.d1) o.d1[col] = (float)other;
+    } else {
+      const double gate = o.gate ? (double)o.gate[col] : 1.0;
+      if (o.d2) o.d2[col] = (float)(t * (o.post_w ? (double)o.post_w[col] : 1.0) + other * (o.post_b ? (double)o.post_b[col] : 0.0));
+      if (o.d3) o.d3[col] = (float)(gate * t);
+      if (o.d4) o.d4[col] = (float)(gate * other);
+    }
   }
 }
 
@@ -398,7 +491,9 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
   a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms; a.res_scale = res_scale; a.eps = eps;
   const int E = dtype == UNETK_BF16 ? 8 : 4;
   const bool vec = C % E == 0 && ldx % E == 0 && ldf % E == 0 && aligned16(x) && aligned16(f) && aligned16(r) && aligned16(n);
-  const unsigned grid = norm_grid(M, C, 4096);
+  // about what the chip holds at once, so that a workgroup has many rows to fetch ahead over (262144 x 96: 43.2 us with
+  // 1536, 50.1 with 4096; 8192 x 4096: 47.9 with 1024, 49.1 with 1536, 53.4 with 4096)
+  const unsigned grid = norm_grid(M, C, norm_shape(C).G > 64 ? 1024 : 1536);
   if (dtype == UNETK_BF16) NORM_DISPATCH(gated_norm_fwd_kernel, bf16);
   else NORM_DISPATCH(gated_norm_fwd_kernel, float);
   UNETK_CHECK_LAUNCH();
@@ -406,7 +501,12 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
 }
 
 int unetk_gated_norm_bwd_rows(int64_t M, int C) {
-  return M < 1 || C < 1 || C > NORM_MAX_C ? 0 : (int)norm_grid(M, C, 1024);
+  // As many workgroups as the chip holds at once (three a CU; two where a row takes several waves and another 10
+  // registers, one where it takes eight): each leaves a row of partials.  65536 x 192: 40.6 us with 768, 55.1 with 256;
+  // 5003 x 1001 fp32: 34.8 with 512, 42.6 with 768; 8192 x 4096: 83.7 with 256, 94.5 with 768.
+  if (M < 1 || C < 1 || C > NORM_MAX_C) return 0;
+  const int G = norm_shape(C).G;
+  return (int)norm_grid(M, C, G > 256 ? 256 : G > 64 ? 512 : 768);
 }
 
 int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t lddn, const void* x, int64_t ldx,
@@ -435,8 +535,8 @@ int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t l
   else NORM_DISPATCH(gated_norm_bwd_kernel, float);
   UNETK_CHECK_LAUNCH();
   if (dgate || dpost_w || dpost_b || dpre_w || dpre_b) {
-    const SumOuts o = {{dpre_w, dpre_b, dgate, dpost_w, dpost_b}};
-    hipLaunchKernelGGL(column_sums_kernel, dim3(cdiv(C, 64), 5), dim3(1024), 0, stream, partials, (int)grid, C, o);
+    const SumArgs o = {dpre_w, dpre_b, dgate, dpost_w, dpost_b, gate, post_w, post_b};
+    hipLaunchKernelGGL(column_sums_kernel, dim3(cdiv(C, 16), 2), dim3(1024), 0, stream, partials, (int)grid, C, o);
     UNETK_CHECK_LAUNCH();
   }
   return UNETK_OK;

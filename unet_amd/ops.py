@@ -941,46 +941,48 @@ def window_attn_bwd(qkv, dout, table, heads, shift, use_mask, defer=None, ws=8):
 # ------------------------------------------------------------------ norms around a branch, 4-bit products
 def _token_rows(t, what, device=None, dtype=None):
     """(rows, row stride) of a channels-last tensor whose rows are equally spaced: a dense tensor, or a channel slice of
-    one."""
+    one.  device: the index it has to have."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
     _require_cuda(t, what)
+    if dtype is not None and t.dtype is not dtype:
+        raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
+    if device is not None and t.get_device() != device:
+        raise ValueError(f"{what}: on {t.device}, expected cuda:{device}")
     if t.dim() < 1:
         raise ValueError(f"{what}: expected (..., channels), got a 0-dim tensor")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what}: on {t.device}, expected {device}")
     C = t.shape[-1]
-    rows = 1
-    for n in t.shape[:-1]:
-        rows *= n
-    if rows * C == 0 or rows == 1:
-        if C > 1 and rows == 1 and t.stride(-1) != 1:
-            raise ValueError(f"{what}: channels must be contiguous (strides {t.stride()})")
-        return rows, max(C, 1)
+    if t.is_contiguous():
+        return (t.numel() // C if C else t[..., None].numel()), max(C, 1)
     # the row axis, outermost first, sizes of one left out: each stride the next one's times its size
     ax = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
-    ld = ax[-1][1]
-    want = ld
+    if C > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: channels must be contiguous (strides {t.stride()})")
+    if not ax:
+        return 1, max(C, 1)
+    ld = want = ax[-1][1]
+    rows = 1
     for n, st in reversed(ax):
         if st != want:
             raise ValueError(f"{what}: rows must be equally spaced (shape {tuple(t.shape)}, strides {t.stride()})")
         want = st * n
-    if (C > 1 and t.stride(-1) != 1) or ld < C:
-        raise ValueError(f"{what}: channels must be contiguous and rows must not overlap (strides {t.stride()})")
+        rows *= n
+    if ld < C:
+        raise ValueError(f"{what}: rows must not overlap (strides {t.stride()})")
     return rows, ld
 
 
 def _vector(t, what, n, device):
+    """Address of a contiguous float32 vector of n on device index ``device`` (None: null)."""
     if t is None:
         return None
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous float32 vector of {n} on {device}, got {t.dtype} "
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_cuda or t.get_device() != device or \
+            not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous float32 vector of {n} on cuda:{device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
-    return t
+    return t.data_ptr()
 
 
 def _norm_pair(p, what, C, device):
@@ -989,28 +991,55 @@ def _norm_pair(p, what, C, device):
     w, b = p
     if w is None:
         raise ValueError(f"{what}: a norm is given by (weight, bias or None)")
-    return _vector(w, what + " weight", C, device), _vector(b, what + " bias", C, device)
+    return _vector(w, what, C, device), _vector(b, what, C, device)
+
+
+class _OnDevice:
+    """Makes device ``index`` the current one for a block; nothing where it is that already (the usual case: torch's own
+    context manager costs the host 3 us)."""
+    __slots__ = ("index", "back")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.back = torch._C._cuda_getDevice()
+        if self.index != self.back:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.back:
+            torch.cuda.set_device(self.back)
+
+
+def _at(t):
+    """Device address for a call, null for None."""
+    return None if t is None else t.data_ptr()
+
+
+_NORM_MAX_C = 8192      # unetk_gated_norm_max_channels()
 
 
 def _gated_norm_args(x, f, gate, keep, post, pre, kind):
-    if kind not in ("layer", "rms"):
+    if kind != "layer" and kind != "rms":
         raise ValueError(f"gated_norm: kind {kind!r} (\"layer\" or \"rms\")")
     M, ldx = _token_rows(x, "x")
-    dtype_code(x.dtype)
+    dev = x.get_device()
     if not isinstance(f, torch.Tensor) or f.shape != x.shape:
         raise ValueError(f"f: expected the shape of x, {tuple(x.shape)}")
-    _, ldf = _token_rows(f, "f", x.device, x.dtype)
+    ldf = _token_rows(f, "f", dev, x.dtype)[1]
     C = x.shape[-1]
-    if not 1 <= C <= _lib.load().unetk_gated_norm_max_channels():
-        raise ValueError(f"gated_norm: {C} channels (1...{_lib.load().unetk_gated_norm_max_channels()})")
-    _vector(gate, "gate", C, x.device)
+    if not 1 <= C <= _NORM_MAX_C:
+        raise ValueError(f"gated_norm: {C} channels (1...{_NORM_MAX_C})")
     rps = 0
     if keep is not None:
         if not isinstance(keep, torch.Tensor) or keep.dim() != 1 or keep.shape[0] < 1 or M % keep.shape[0]:
             raise ValueError(f"keep: expected one factor a sample for {M} rows")
-        _vector(keep, "keep", keep.shape[0], x.device)
         rps = M // keep.shape[0]
-    return M, C, ldx, ldf, rps, _norm_pair(post, "post", C, x.device), _norm_pair(pre, "pre", C, x.device)
+        keep = _vector(keep, "keep", keep.shape[0], dev)
+    qw, qb = _norm_pair(post, "post", C, dev)
+    pw, pb = _norm_pair(pre, "pre", C, dev)
+    return M, C, dev, ldx, ldf, dtype_code(x.dtype), _vector(gate, "gate", C, dev), keep, rps, qw, qb, pw, pb
 
 
 def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=None, kind="layer", eps=1e-5, want_stats=True):
@@ -1023,15 +1052,14 @@ def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=Non
     the mean).  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
     float32.  Returns (r, n, stats): r and n dense, n None without pre; stats is what gated_norm_bwd reads (None unless
     want_stats).  n is taken from the unrounded r."""
-    M, C, ldx, ldf, rps, (qw, qb), (pw, pb) = _gated_norm_args(x, f, gate, keep, post, pre, kind)
-    with torch.cuda.device(x.device):
+    M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
+    with _OnDevice(dev):
         r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         n = torch.empty_like(r) if pw is not None else None
         stats = torch.empty((M, 4), dtype=torch.float32, device=x.device) if want_stats else None
         if M:
-            call("unetk_gated_norm_fwd", ptr(x), ldx, ptr(f), ldf, ptr(gate), ptr(keep), rps, float(res_scale), ptr(qw),
-                 ptr(qb), ptr(pw), ptr(pb), int(kind == "rms"), float(eps), ptr(r), ptr(n), ptr(stats), M, C,
-                 dtype_code(x.dtype), stream())
+            call("unetk_gated_norm_fwd", x.data_ptr(), ldx, f.data_ptr(), ldf, g, keep, rps, res_scale, qw, qb, pw, pb,
+                 kind == "rms", eps, r.data_ptr(), _at(n), _at(stats), M, C, code, stream())
     return r, n, stats
 
 
@@ -1050,34 +1078,38 @@ def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, pos
     """Gradients of gated_norm_fwd (the same arguments, and its stats) from dr and dn, the gradients of r and n.  dr may
     be None where nothing else reads r; dn is given exactly when pre is.  Sums over rows are taken in a fixed order: the
     same bits every time."""
-    M, C, ldx, ldf, rps, (qw, qb), (pw, pb) = _gated_norm_args(x, f, gate, keep, post, pre, kind)
+    M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
     if (dn is None) != (pw is None) or (dr is None and dn is None):
         raise ValueError("gated_norm_bwd: dn goes with pre, and one of dr and dn has to be there")
-    ld = []
-    for g, what in ((dr, "dr"), (dn, "dn")):
-        if g is not None and (not isinstance(g, torch.Tensor) or g.shape != x.shape):
+    lddr = lddn = 0
+    for t, what in ((dr, "dr"), (dn, "dn")):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != x.shape):
             raise ValueError(f"{what}: expected the shape of x, {tuple(x.shape)}")
-        ld.append(0 if g is None else _token_rows(g, what, x.device, x.dtype)[1])
-    if not isinstance(stats, torch.Tensor) or stats.shape != (M, 4) or stats.dtype != torch.float32 or \
-            stats.device != x.device or not stats.is_contiguous():
+    if dr is not None:
+        lddr = _token_rows(dr, "dr", dev, x.dtype)[1]
+    if dn is not None:
+        lddn = _token_rows(dn, "dn", dev, x.dtype)[1]
+    if not isinstance(stats, torch.Tensor) or stats.shape != (M, 4) or stats.dtype is not torch.float32 or \
+            not stats.is_cuda or stats.get_device() != dev or not stats.is_contiguous() or stats.data_ptr() % 16:
         raise ValueError(f"stats: expected what gated_norm_fwd returned for these {M} rows")
-    dev = x.device
-    with torch.cuda.device(dev):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    device = x.device
+    with _OnDevice(dev):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device)
         df = torch.empty_like(dx)
-        dgate, dqw, dqb, dpw, dpb = (None if p is None else torch.empty(C, dtype=torch.float32, device=dev)
-                                     for p in (gate, qw, qb, pw, pb))
+        # one block for the parameters' gradients: pre weight, pre bias, gate, post weight, post bias
+        there = (pw, pb, g, qw, qb)
+        block = torch.empty((sum(p is not None for p in there), C), dtype=torch.float32, device=device)
+        rows = iter(block.unbind(0))
+        dpw, dpb, dg, dqw, dqb = (None if p is None else next(rows) for p in there)
         if M:
-            rows = _lib.load().unetk_gated_norm_bwd_rows(M, C)
-            partials = torch.empty((rows, 5, C), dtype=torch.float32, device=dev)
-            call("unetk_gated_norm_bwd", ptr(dr), ld[0], ptr(dn), ld[1], ptr(x), ldx, ptr(f), ldf, ptr(stats), ptr(gate),
-                 ptr(keep), rps, float(res_scale), ptr(qw), ptr(qb), ptr(pw), int(kind == "rms"), ptr(dx), ptr(df),
-                 ptr(dgate), ptr(dqw), ptr(dqb), ptr(dpw), ptr(dpb), ptr(partials), M, C, dtype_code(x.dtype), stream())
+            lib = _lib.load()
+            partials = torch.empty(lib.unetk_gated_norm_bwd_rows(M, C) * 4 * C, dtype=torch.float32, device=device)
+            call("unetk_gated_norm_bwd", _at(dr), lddr, _at(dn), lddn, x.data_ptr(), ldx, f.data_ptr(), ldf, stats.data_ptr(),
+                 g, keep, rps, res_scale, qw, qb, pw, kind == "rms", dx.data_ptr(), df.data_ptr(), _at(dg), _at(dqw),
+                 _at(dqb), _at(dpw), _at(dpb), partials.data_ptr(), M, C, code, stream())
         else:
-            for g in (dgate, dqw, dqb, dpw, dpb):
-                if g is not None:
-                    g.zero_()
-    return GatedNormGrads(dx, df, dgate, dqw, dqb, dpw, dpb)
+            block.zero_()
+    return GatedNormGrads(dx, df, dg, dqw, dqb, dpw, dpb)
 
 
 class MxTensor:
@@ -1113,14 +1145,14 @@ def mx_quantize(x) -> MxTensor:
     if K < 1:
         raise ValueError("mx_quantize: no elements to scale (K = 0)")
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    with _OnDevice(x.get_device()):
         nc = lib.unetk_mx_codes_bytes(rows, K) if rows else 0
         if rows and not nc:
             raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
         codes = torch.empty(nc, dtype=torch.uint8, device=x.device)
         scales = torch.empty(nc // 16, dtype=torch.uint8, device=x.device)
         if rows:
-            call("unetk_mx_quantize", ptr(x), ld, rows, K, code, ptr(codes), ptr(scales), stream())
+            call("unetk_mx_quantize", _at(x), ld, rows, K, code, _at(codes), _at(scales), stream())
     return MxTensor(codes, scales, x.shape)
 
 
@@ -1129,10 +1161,10 @@ def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
     if not isinstance(q, MxTensor):
         raise TypeError(f"mx_dequantize: expected an MxTensor, got {type(q).__name__}")
     code, rows, K = dtype_code(dtype), q.rows, q.shape[-1]
-    with torch.cuda.device(q.device):
+    with _OnDevice(q.device.index):
         out = torch.empty(q.shape, dtype=dtype, device=q.device)
         if rows:
-            call("unetk_mx_dequantize", ptr(q.codes), ptr(q.scales), rows, K, ptr(out), K, code, stream())
+            call("unetk_mx_dequantize", _at(q.codes), _at(q.scales), rows, K, _at(out), K, code, stream())
     return out
 
 
@@ -1161,20 +1193,20 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
             raise ValueError(f"mx_linear: dtype {dtype} for x of {x.dtype}")
         dt, rows = x.dtype, _token_rows(x, "x")[0]
     code, shape, dev = dtype_code(dt), x.shape[:-1] + (N,), w.device
-    _vector(bias, "bias", N, dev)
+    bias = _vector(bias, "bias", N, dev.index)
     ldo = ldr = N
     for t, what in ((out, "out"), (resid, "resid")):
         if t is not None and (not isinstance(t, torch.Tensor) or t.shape != shape):
             raise ValueError(f"{what}: expected the shape {tuple(shape)}")
     if out is not None:
-        ldo = _token_rows(out, "out", dev, dt)[1]
+        ldo = _token_rows(out, "out", dev.index, dt)[1]
     if resid is not None:
-        ldr = _token_rows(resid, "resid", dev, dt)[1]
-    with torch.cuda.device(dev):
+        ldr = _token_rows(resid, "resid", dev.index, dt)[1]
+    with _OnDevice(dev.index):
         if out is None:
             out = torch.empty(shape, dtype=dt, device=dev)
         if rows and N:
             xq = x if quantised else mx_quantize(x)
-            call("unetk_mx_linear", ptr(xq.codes), ptr(xq.scales), ptr(w.codes), ptr(w.scales), ptr(out), ldo, rows, K, N,
-                 ptr(bias), act, ptr(resid), ldr, code, stream())
+            call("unetk_mx_linear", _at(xq.codes), _at(xq.scales), _at(w.codes), _at(w.scales), _at(out), ldo, rows, K, N,
+                 bias, act, _at(resid), ldr, code, stream())
     return out
