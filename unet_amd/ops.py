@@ -1191,7 +1191,8 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
     else:
         if dtype is not None and dtype != x.dtype:
             raise ValueError(f"mx_linear: dtype {dtype} for x of {x.dtype}")
-        dt, rows = x.dtype, _token_rows(x, "x")[0]
+        dt = x.dtype
+        rows, ldx = _token_rows(x, "x")
     code, shape, dev = dtype_code(dt), x.shape[:-1] + (N,), w.device
     bias = _vector(bias, "bias", N, dev.index)
     ldo = ldr = N
@@ -1206,7 +1207,13 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
         if out is None:
             out = torch.empty(shape, dtype=dt, device=dev)
         if rows and N:
-            xq = x if quantised else mx_quantize(x)
-            call("unetk_mx_linear", _at(xq.codes), _at(xq.scales), _at(w.codes), _at(w.scales), _at(out), ldo, rows, K, N,
-                 bias, act, _at(resid), ldr, code, stream())
+            lib = _lib.load()
+            if not quantised and ldx * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0 and \
+                    lib.unetk_mx_linear_x_supported(rows, K, N, code):
+                call("unetk_mx_linear_x", x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, rows,
+                     K, N, bias, act, _at(resid), ldr, code, stream())
+            else:
+                xq = x if quantised else mx_quantize(x)
+                call("unetk_mx_linear", xq.codes.data_ptr(), xq.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+                     out.data_ptr(), ldo, rows, K, N, bias, act, _at(resid), ldr, code, stream())
     return out
