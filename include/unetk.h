@@ -443,13 +443,13 @@ int unetk_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int d
 int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int64_t ldo, int dtype,
                         unetk_stream_t stream);
 /* out[m][n] = act(sum_k x[m][k] * w[n][k] + bias[n]) + resid[m][n], both operands quantised: x (M, K), w (N, K).
- * bias: N floats or null; act: 0 none, 1 ReLU, 2 GELU (erf form); resid: rows of N elements of `dtype`, ldr apart, or
+ * bias: N floats or null; act: 0 none, 2 GELU (erf form); resid: rows of N elements of `dtype`, ldr apart, or
  * null; out: rows ldo apart.  Sums in fp32. */
 int unetk_mx_linear(const void* xcodes, const void* xscales, const void* wcodes, const void* wscales, void* out, int64_t ldo,
                     int64_t M, int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
                     unetk_stream_t stream);
 
-/* The same from unquantised activations (M rows of K elements of `dtype`, ldx apart, 16-byte aligned rows) in one launch,
+/* The same from unquantised activations (M rows of K elements of `dtype`, ldx apart) in one launch,
  * for the problems that unetk_mx_linear_x_supported names: few rows, or short K under many rows.  Same bits as
  * unetk_mx_quantize followed by unetk_mx_linear. */
 int unetk_mx_linear_x_supported(int64_t M, int64_t K, int64_t N, int dtype);

@@ -118,7 +118,7 @@ def check_linear(rows, K, N, dt, bias=True, act=0, resid=True, x=None, scale=1.0
     want, mag = xv @ wv.t(), xv.abs() @ wv.abs().t()
     if b is not None:
         want, mag = want + b.cuda().double(), mag + b.cuda().double().abs()
-    want = gelu(want) if act == 2 else want.clamp_min(0) if act == 1 else want
+    want = gelu(want) if act == 2 else want
     if r is not None:
         want, mag = want + r.cuda().double(), mag + r.cuda().double().abs()
     assert got.shape == (rows, N) and got.dtype == dt
@@ -141,7 +141,7 @@ def test_product(rows, K, N, dt):
     check_linear(rows, K, N, dt)
 
 
-@pytest.mark.parametrize("act", [0, 1, 2])
+@pytest.mark.parametrize("act", [0, 2])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("resid", [False, True])
 def test_epilogues(act, bias, resid):
@@ -244,7 +244,7 @@ def test_refusals():
     qw = ops.mx_quantize(w)
     for f in (lambda: ops.mx_quantize(x.half()), lambda: ops.mx_quantize(x.t()), lambda: ops.mx_quantize(x[:, :0]),
               lambda: ops.mx_dequantize(qw, torch.float16), lambda: ops.mx_linear(x[:, :64], qw),
-              lambda: ops.mx_linear(x, qw, bias=torch.zeros(39, device="cuda")), lambda: ops.mx_linear(x, qw, act=3),
+              lambda: ops.mx_linear(x, qw, bias=torch.zeros(39, device="cuda")), lambda: ops.mx_linear(x, qw, act=1),
               lambda: ops.mx_linear(x, qw, resid=torch.zeros((4, 39), device="cuda")),
               lambda: ops.mx_linear(x, qw, resid=torch.zeros((4, 40), device="cuda", dtype=BF)),
               lambda: ops.mx_linear(x, qw, out=torch.zeros((40, 4), device="cuda").t()),

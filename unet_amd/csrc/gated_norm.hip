@@ -12,7 +12,7 @@
 // operations an element.  All arithmetic is fp32; r, n, dx, df are rounded once, when they are stored.  n comes from the
 // unrounded r (which is in registers), and the backward pass forms r again from x and f for the same reason: it reads
 // as many bytes as with a stored r.
-#include "common.h"
+#include "unaligned.h"
 
 namespace {
 
@@ -33,26 +33,28 @@ struct NormArgs {
   float res_scale, eps;
 };
 
-// The elements of a row that one of its G lanes holds: N = NV 16-byte vectors.  Whole vectors where rows are 16-byte
-// aligned (VEC), else single elements with neighbouring lanes on neighbouring channels.
-template <typename T, int G, int NV, bool VEC> struct Lane {
+// The elements of a row that one of its G lanes holds: N = NV 16-byte vectors, at whatever address the row begins.
+// WHOLE: C is a multiple of the vector's elements; else the lanes take single elements side by side (20000 x 1001 bf16
+// forward: 44.4 us so, 59.2 with vectors off their alignment; 5003 x 1001 fp32: 17.2 and 22.0).
+template <typename T, int G, int NV, bool WHOLE> struct Lane {
   static constexpr int E = Vec16<T>::N, N = NV * E;
+  static constexpr bool SINGLE = !WHOLE;
   int gl, C;
-  __device__ __forceinline__ int chan(int i) const { return VEC ? ((i / E) * G + gl) * E + i % E : i * G + gl; }
-  __device__ __forceinline__ bool has(int i) const { return (VEC ? ((i / E) * G + gl) * E : i * G + gl) < C; }
+  __device__ __forceinline__ int chan(int i) const { return SINGLE ? i * G + gl : ((i / E) * G + gl) * E + i % E; }
+  __device__ __forceinline__ bool has(int i) const { return WHOLE ? ((i / E) * G + gl) * E < C : chan(i) < C; }
   struct Raw {
     Vec16<T> v[NV];
   };
   __device__ __forceinline__ void load(Raw& r, const T* row) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      r.v[k] = zero16<T>();
-      if (VEC) {
-        if (has(k * E)) r.v[k] = load16(row + chan(k * E));
-      } else {
+      if (SINGLE) {
+        r.v[k] = zero16<T>();
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (has(k * E + e)) r.v[k].v[e] = row[chan(k * E + e)];
+      } else {
+        r.v[k] = load_part<true>(row + chan(k * E), C - chan(k * E));
       }
     }
   }
@@ -60,15 +62,15 @@ template <typename T, int G, int NV, bool VEC> struct Lane {
   __device__ __forceinline__ void store(T* row, const float (&d)[N]) const {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if (VEC) {
-        Vec16<T> o;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(d[k * E + e]);
-        if (has(k * E)) store16(row + chan(k * E), o);
-      } else {
+      if (SINGLE) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (has(k * E + e)) row[chan(k * E + e)] = from_f32<T>(d[k * E + e]);
+      } else {
+        Vec16<T> o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(d[k * E + e]);
+        store_part<true>(row + chan(k * E), o, C - chan(k * E));
       }
     }
   }
@@ -163,9 +165,9 @@ __device__ __forceinline__ float residual(float x, float fhat, float gw, float g
   return fmaf(keep, fmaf(fhat, gw, gb), x * scale);
 }
 
-template <typename T, int G, int NV, bool VEC>
+template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs a) {
-  using L = Lane<T, G, NV, VEC>;
+  using L = Lane<T, G, NV, WHOLE>;
   constexpr int N = L::N, RPB = threads_of(G) / G;
   __shared__ float red[2][2][threads_of(G) / 64];
   RowSum<G> rs{red};
@@ -226,9 +228,9 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
 // w_post and b_post are these times constants of the channel: dgate = w_post sum(u fhat) + b_post sum(u), dw_post = gate
 // sum(u fhat), db_post = gate sum(u).  The sums leave as one [4][C] row of partials a workgroup, added in a fixed order by
 // column_sums_kernel: no atomics, the same bits every time.
-template <typename T, int G, int NV, bool VEC>
+template <typename T, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs a) {
-  using L = Lane<T, G, NV, VEC>;
+  using L = Lane<T, G, NV, WHOLE>;
   constexpr int N = L::N, RPB = threads_of(G) / G;
   __shared__ float red[2][2][threads_of(G) / 64];
   __shared__ float xch[RPB > 1 ? threads_of(G) * N : 1];
@@ -435,29 +437,27 @@ unsigned norm_grid(int64_t M, int C, int cap) {
   return (unsigned)(b < cap ? b : cap);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-#define NORM_LAUNCH(KERNEL, T, G_, K_, VEC_)                                                                  \
-  hipLaunchKernelGGL((KERNEL<T, G_, K_ * (8 / Vec16<T>::N), VEC_>), dim3(grid), dim3(threads_of(G_)), 0, stream, a)
-#define NORM_VEC(KERNEL, T, G_, K_)              \
+#define NORM_LAUNCH(KERNEL, T, G_, K_, WHOLE_)                                                                  \
+  hipLaunchKernelGGL((KERNEL<T, G_, K_ * (8 / Vec16<T>::N), WHOLE_>), dim3(grid), dim3(threads_of(G_)), 0, stream, a)
+#define NORM_TAIL(KERNEL, T, G_, K_)              \
   do {                                           \
-    if (vec) NORM_LAUNCH(KERNEL, T, G_, K_, true); \
+    if (whole) NORM_LAUNCH(KERNEL, T, G_, K_, true); \
     else NORM_LAUNCH(KERNEL, T, G_, K_, false);  \
   } while (0)
 #define NORM_DISPATCH(KERNEL, T)                                   \
   do {                                                             \
     const Shape sh = norm_shape(a.C);                              \
     switch (sh.G) {                                                \
-      case 4: NORM_VEC(KERNEL, T, 4, 1); break;                    \
-      case 8: NORM_VEC(KERNEL, T, 8, 1); break;                    \
-      case 16: NORM_VEC(KERNEL, T, 16, 1); break;                  \
-      case 32: NORM_VEC(KERNEL, T, 32, 1); break;                  \
-      case 64: NORM_VEC(KERNEL, T, 64, 1); break;                  \
-      case 128: NORM_VEC(KERNEL, T, 128, 1); break;                \
-      case 256: NORM_VEC(KERNEL, T, 256, 1); break;                \
+      case 4: NORM_TAIL(KERNEL, T, 4, 1); break;                    \
+      case 8: NORM_TAIL(KERNEL, T, 8, 1); break;                    \
+      case 16: NORM_TAIL(KERNEL, T, 16, 1); break;                  \
+      case 32: NORM_TAIL(KERNEL, T, 32, 1); break;                  \
+      case 64: NORM_TAIL(KERNEL, T, 64, 1); break;                  \
+      case 128: NORM_TAIL(KERNEL, T, 128, 1); break;                \
+      case 256: NORM_TAIL(KERNEL, T, 256, 1); break;                \
       default:                                                     \
-        if (sh.K == 1) NORM_VEC(KERNEL, T, 512, 1);                \
-        else NORM_VEC(KERNEL, T, 512, 2);                          \
+        if (sh.K == 1) NORM_TAIL(KERNEL, T, 512, 1);                \
+        else NORM_TAIL(KERNEL, T, 512, 2);                          \
     }                                                              \
   } while (0)
 
@@ -489,8 +489,7 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
   a.x = x; a.f = f; a.ldx = ldx; a.ldf = ldf; a.gate = gate; a.keep = keep; a.post_w = post_w; a.post_b = post_b;
   a.pre_w = pre_w; a.pre_b = pre_b; a.stats_out = stats; a.o0 = r; a.o1 = n; a.M = (uint32_t)M;
   a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms; a.res_scale = res_scale; a.eps = eps;
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  const bool vec = C % E == 0 && ldx % E == 0 && ldf % E == 0 && aligned16(x) && aligned16(f) && aligned16(r) && aligned16(n);
+  const bool whole = C % (dtype == UNETK_BF16 ? 8 : 4) == 0;
   // about what the chip holds at once, so that a workgroup has many rows to fetch ahead over (262144 x 96: 43.2 us with
   // 1536, 50.1 with 4096; 8192 x 4096: 47.9 with 1024, 49.1 with 1536, 53.4 with 4096)
   const unsigned grid = norm_grid(M, C, norm_shape(C).G > 64 ? 1024 : 1536);
@@ -527,9 +526,7 @@ int unetk_gated_norm_bwd(const void* dr, int64_t lddr, const void* dn, int64_t l
   a.keep = keep; a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.stats_in = stats; a.o0 = dx; a.o1 = df;
   a.partials = partials; a.M = (uint32_t)M; a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms;
   a.res_scale = res_scale;
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  const bool vec = C % E == 0 && ldx % E == 0 && ldf % E == 0 && (!dr || lddr % E == 0) && (!dn || lddn % E == 0) &&
-                   aligned16(x) && aligned16(f) && aligned16(dr) && aligned16(dn) && aligned16(dx) && aligned16(df);
+  const bool whole = C % (dtype == UNETK_BF16 ? 8 : 4) == 0;
   const unsigned grid = (unsigned)unetk_gated_norm_bwd_rows(M, C);
   if (dtype == UNETK_BF16) NORM_DISPATCH(gated_norm_bwd_kernel, bf16);
   else NORM_DISPATCH(gated_norm_bwd_kernel, float);

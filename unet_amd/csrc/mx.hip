@@ -6,21 +6,26 @@
 // elements are x / 2^se rounded half to even and held to 6.  A block with a NaN or an infinity gets the scale byte 255 (NaN):
 // everything made from it is NaN.
 //
-// Layout: the one the matrix instruction reads, for both operands.  v_mfma_scale_f32_16x16x128_f8f6f4 takes of each
-// operand 16 rows x 128 k; lane l holds row l % 16, k block l / 16: 32 consecutive elements, 16 bytes, exactly one block,
-// and in one byte that block's scale.  Rows are padded to 64, K to 128 (zero elements, scale byte 0), and stored as
+// Layout: the one the matrix instruction reads, for both operands.  v_mfma_scale_f32_32x32x64_f8f6f4 takes of each operand
+// 32 rows x 64 k; lane l holds row l % 32, k block l / 32: 32 consecutive elements, 16 bytes, exactly one block, and in one
+// byte that block's scale.  (The 16x16x128 shape multiplies at 5.0...6.4 PFLOP/s here, this one at 9.3.)  Rows are padded to
+// 64, K to 128 (zero elements, scale byte 0), and stored in units of 64 rows x 128 k:
 //   codes  [rows/64][K/128][4 fragments][64 lanes][16 bytes]     (element j of a block in nibble j, low nibble first)
 //   scales [rows/64][K/128][64 lanes][4 bytes]                   (byte f: the lane's block of fragment f)
-// so that a fragment is 1 KB and the scales of four are 256 bytes, read without a gap.  Row r of fragment f is row
-// 32 (f / 2) + 8 (r / 4) + 4 (f % 2) + r % 4 of its 64: with the weights as the instruction's first operand, whose rows come
-// out four to a lane, the accumulators of two fragments are then 8 consecutive output columns of one row.
+// fragment f: rows 32 (f % 2) + ..., k 64 (f / 2) + ..., so that a fragment is 1 KB and the scales of four are 256 bytes, read
+// without a gap.  Row r of a fragment is row 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4 of its 32: with the weights as the
+// instruction's first operand, whose rows come out in fours eight apart, a lane's accumulators are then two runs of 8
+// consecutive output columns of one row.
 #include "epilogue.h"
+#include "unaligned.h"
 
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ int frag_row(int f, int r) { return ((f >> 1) << 5) + ((r >> 2) << 3) + ((f & 1) << 2) + (r & 3); }
+// row of a fragment's 32 (or the other way round: the map is its own inverse)
+__device__ __forceinline__ int frag_row(int r) { return (r & 16) + ((r & 4) << 1) + ((r & 8) >> 1) + (r & 3); }
 
 // 32 values -> 32 codes and the scale byte.  Everything is exact but the rounding itself (the scale is a power of two), and
 // the conversion instructions do that rounding: half to even, held to 6, for every scale byte from 0 on.
@@ -80,25 +85,16 @@ __device__ __forceinline__ uint32_t mx_block(const RawBlock<float>& x, u32x4& co
 }
 
 // 32 consecutive elements of a row, zeros past its end (and for a row that is not there)
-template <typename T, bool VEC>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void load_block(const T* row, int k0, int K, bool there, RawBlock<T>& x) {
   constexpr int E = Vec16<T>::N;
 #pragma unroll
-  for (int j = 0; j < RawBlock<T>::N; ++j) {
-    Vec16<T> r = zero16<T>();
-    if (VEC) {
-      if (there && k0 + j * E < K) r = load16(row + k0 + j * E);
-    } else if (there) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (k0 + j * E + e < K) r.v[e] = row[k0 + j * E + e];
-    }
-    x.v[j] = __builtin_bit_cast(u32x4, r);
-  }
+  for (int j = 0; j < RawBlock<T>::N; ++j)
+    x.v[j] = __builtin_bit_cast(u32x4, load_part<WHOLE>(row + k0 + j * E, there ? K - (k0 + j * E) : 0));
 }
 
 // One wave: 64 rows x 128 k, each lane whole blocks.  Bound by the read of x.
-template <typename T, bool VEC>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t rows, int K,
                                                           uint32_t kt, uint64_t units, u32x4* __restrict__ codes,
                                                           uint32_t* __restrict__ scales) {
@@ -106,13 +102,13 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
   if (unit >= units) return;
   const int lane = threadIdx.x & 63;
   const uint32_t g = (uint32_t)(unit / kt);
-  const int k0 = (int)(unit % kt) * 128 + (lane >> 4) * 32;
+  const int k0 = (int)(unit % kt) * 128 + (lane >> 5) * 32;
   uint32_t sc = 0;
 #pragma unroll
   for (int f = 0; f < 4; ++f) {
-    const uint32_t row = g * 64 + frag_row(f, lane & 15);
+    const uint32_t row = g * 64 + (f & 1) * 32 + frag_row(lane & 31);
     RawBlock<T> r;
-    load_block<T, VEC>(x + (int64_t)(row < rows ? row : 0) * ldx, k0, K, row < rows, r);
+    load_block<T, WHOLE>(x + (int64_t)(row < rows ? row : 0) * ldx, k0 + (f >> 1) * 64, K, row < rows, r);
     u32x4 c;
     sc |= mx_block(r, c) << (8 * f);
     codes[(unit * 4 + f) * 64 + lane] = c;
@@ -132,39 +128,28 @@ __device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
   return (code & 8u) ? -v : v;
 }
 
-template <typename T>
+// One wave: one fragment (32 rows x 64 k).  Bound by the write of the values.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const u32x4* __restrict__ codes, const uint32_t* __restrict__ scales,
-                                                            uint32_t rows, int K, uint32_t kt, uint64_t units,
-                                                            T* __restrict__ out, int64_t ldo, int vec) {
-  const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= units) return;
+                                                            uint32_t rows, int K, uint32_t kt, T* __restrict__ out, int64_t ldo) {
   constexpr int E = Vec16<T>::N;
-  const int lane = threadIdx.x & 63;
-  const uint32_t g = (uint32_t)(unit / kt);
-  const int k0 = (int)(unit % kt) * 128 + (lane >> 4) * 32;
-  const uint32_t sc = scales[unit * 64 + lane];
+  const uint64_t unit = blockIdx.x;
+  const int lane = threadIdx.x & 63, f = threadIdx.x >> 6;
+  const uint32_t row = (uint32_t)(unit / kt) * 64 + (f & 1) * 32 + frag_row(lane & 31);
+  const int k0 = (int)(unit % kt) * 128 + (f >> 1) * 64 + (lane >> 5) * 32;
+  if (row >= rows) return;
+  const u32x4 c = codes[(unit * 4 + f) * 64 + lane];
+  const uint32_t sc = scales[unit * 64 + lane] >> (8 * f) & 255u;
+  T* o = out + (int64_t)row * ldo + k0;
 #pragma unroll
-  for (int f = 0; f < 4; ++f) {
-    const uint32_t row = g * 64 + frag_row(f, lane & 15);
-    if (row >= rows) continue;
-    const u32x4 c = codes[(unit * 4 + f) * 64 + lane];
-    T* o = out + (int64_t)row * ldo + k0;
+  for (int j = 0; j < 32 / E; ++j) {
+    Vec16<T> v;
 #pragma unroll
-    for (int j = 0; j < 32 / E; ++j) {
-      Vec16<T> v;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = j * E + e;
-        v.v[e] = from_f32<T>(mx_value(c[i / 8] >> (4 * (i % 8)), (sc >> (8 * f)) & 255u));
-      }
-      if (vec) {
-        if (k0 + j * E < K) store16(o + j * E, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (k0 + j * E + e < K) o[j * E + e] = v.v[e];
-      }
+    for (int e = 0; e < E; ++e) {
+      const int i = j * E + e;
+      v.v[e] = from_f32<T>(mx_value(c[i / 8] >> (4 * (i % 8)), sc));
     }
+    store_part<WHOLE>(o + j * E, v, K - (k0 + j * E));
   }
 }
 
@@ -177,17 +162,26 @@ struct MxArgs {
   const void* resid;
   int64_t ldx, ldo, ldr;
   uint32_t M, N, kt;      // rows, output columns, steps of 128 k
-  int K, act, vec;
+  int K, act, whole;
   uint32_t ngroups, per;  // mx_rows_kernel: groups of 64 columns, and how many of them a workgroup takes
 };
 
-// fragments FW of the weights and FX of the activations (their scales: byte FW / FX of the lane's word)
+// a fragment of the weights and one of the activations (their scales: bytes FW / FX of the lane's words)
 template <int FW, int FX>
-__device__ __forceinline__ f32x4 mma4(const u32x4& w, const u32x4& x, f32x4 c, uint32_t sw, uint32_t sx) {
+__device__ __forceinline__ f32x16 mma32(const u32x4& w, const u32x4& x, f32x16 c, uint32_t sw, uint32_t sx) {
 #if defined(__HIP_DEVICE_COMPILE__)
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
   const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, FW, (int)sw, FX, (int)sx);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 4, 4, FW, (int)sw, FX, (int)sx);
+#else
+  return c;
+#endif
+}
+__device__ __forceinline__ f32x4 mma16(const u32x4& w, const u32x4& x, f32x4 c, uint32_t sw, uint32_t sx) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, (int)sw, 0, (int)sx);
 #else
   return c;
 #endif
@@ -210,28 +204,25 @@ __device__ __forceinline__ float gelu_bf16(float v) {
   return fmaf(-a, __builtin_amdgcn_exp2f(p), v < 0.f ? 0.f : v);
 }
 
-template <typename T, int ACT> __device__ __forceinline__ float mx_act(float v) {
-  if (ACT == 1) return v < 0.f ? 0.f : v;
-  if (ACT == 2) return sizeof(T) == 2 ? gelu_bf16(v) : 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
-  return v;
+template <typename T, bool GELU> __device__ __forceinline__ float mx_act(float v) {
+  if (!GELU) return v;
+  return sizeof(T) == 2 ? gelu_bf16(v) : 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
 }
 
-// The columns of a lane's accumulators: pair j of fragments (2j, 2j + 1) holds columns n0 + 32 j + 8 (lane / 16) + 0...7
-// of one row.  Accumulators begin as the bias.
-__device__ __forceinline__ f32x4 bias4(const MxArgs& a, uint32_t n0, int f, int lane) {
-  const uint32_t n = n0 + ((f >> 1) << 5) + ((lane >> 4) << 3) + ((f & 1) << 2);
-  f32x4 b = {0.f, 0.f, 0.f, 0.f};
-  if (a.bias != nullptr) {
+// Accumulators begin as the bias: run j (of two) of a 32-column fragment at n0 is columns n0 + 16 j + 8 (lane / 32) + 0...7.
+__device__ __forceinline__ f32x16 bias16(const MxArgs& a, uint32_t n0, int lane) {
+  f32x16 b;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) b[i] = a.bias[n + i];
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t n = n0 + ((i >> 3) << 4) + ((lane >> 5) << 3) + (i & 7);
+    b[i] = (a.bias != nullptr && n < a.N) ? a.bias[n] : 0.f;
   }
   return b;
 }
 
-// activation, residual and store of 8 consecutive columns of row m (lo, hi: accumulators of two fragments)
-template <typename T, int ACT, bool VEC>
-__device__ __forceinline__ void store8(const MxArgs& a, uint32_t m, uint32_t n, const f32x4& lo, const f32x4& hi) {
+// activation, residual and store of run J of a fragment: 8 consecutive columns, from n on, of row m
+template <typename T, bool ACT, bool WHOLE, int J>
+__device__ __forceinline__ void store8(const MxArgs& a, uint32_t m, uint32_t n, const f32x16& acc) {
   constexpr int E = Vec16<T>::N;
   if (m >= a.M) return;
   T* o = reinterpret_cast<T*>(a.out) + (int64_t)m * a.ldo + n;
@@ -239,96 +230,155 @@ __device__ __forceinline__ void store8(const MxArgs& a, uint32_t m, uint32_t n, 
   for (int j = 0; j < 8 / E; ++j) {
     float y[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = mx_act<T, ACT>(j * E + e < 4 ? lo[(j * E + e) % 4] : hi[(j * E + e) % 4]);
+    for (int e = 0; e < E; ++e) y[e] = mx_act<T, ACT>(acc[J * 8 + j * E + e]);
+    const int left = (int)(a.N - n) - j * E;      // (n may lie past the last column: below zero)
     if (a.resid != nullptr) {
-      const T* rs = reinterpret_cast<const T*>(a.resid) + (int64_t)m * a.ldr + n + j * E;
-      if (VEC) {
-        if (n + j * E < a.N) {
-          const Vec16<T> r = load16(rs);
+      const Vec16<T> r = load_part<WHOLE>(reinterpret_cast<const T*>(a.resid) + (int64_t)m * a.ldr + n + j * E, left);
 #pragma unroll
-          for (int e = 0; e < E; ++e) y[e] += to_f32(r.v[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (n + j * E + e < a.N) y[e] += to_f32(rs[e]);
-      }
+      for (int e = 0; e < E; ++e) y[e] += to_f32(r.v[e]);
     }
-    if (VEC) {
-      Vec16<T> v;
+    Vec16<T> v;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(y[e]);
-      if (n + j * E < a.N) store16(o + j * E, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (n + j * E + e < a.N) o[j * E + e] = from_f32<T>(y[e]);
-    }
+    for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(y[e]);
+    store_part<WHOLE>(o + j * E, v, left);
   }
 }
 
-// f(activation, whole 16-byte stores or not) as constants: the branch is taken once a tile, not once an element
+// a 32 x 32 tile: row m (this lane's), columns n0 + ...
+template <typename T, bool ACT, bool WHOLE>
+__device__ __forceinline__ void store_tile(const MxArgs& a, uint32_t m, uint32_t n0, int lane, const f32x16& acc) {
+  const uint32_t n = n0 + ((lane >> 5) << 3);
+  store8<T, ACT, WHOLE, 0>(a, m, n, acc);
+  store8<T, ACT, WHOLE, 1>(a, m, n + 16, acc);
+}
+
+// f(GELU or not, rows of whole 16-byte pieces or not) as constants: the branch is taken once a tile, not once an element
 template <typename F> __device__ __forceinline__ void with_epilogue(const MxArgs& a, F&& f) {
-  using std::integral_constant;
-  if (a.vec) {
-    if (a.act == 0) f(integral_constant<int, 0>{}, integral_constant<bool, true>{});
-    else if (a.act == 1) f(integral_constant<int, 1>{}, integral_constant<bool, true>{});
-    else f(integral_constant<int, 2>{}, integral_constant<bool, true>{});
+  std::integral_constant<bool, false> no;
+  std::integral_constant<bool, true> yes;
+  if (a.whole) {
+    if (a.act == 0) f(no, yes);
+    else f(yes, yes);
   } else {
-    if (a.act == 0) f(integral_constant<int, 0>{}, integral_constant<bool, false>{});
-    else if (a.act == 1) f(integral_constant<int, 1>{}, integral_constant<bool, false>{});
-    else f(integral_constant<int, 2>{}, integral_constant<bool, false>{});
+    if (a.act == 0) f(no, no);
+    else f(yes, no);
   }
 }
 
-// ---- few tiles: the W waves of a workgroup share the steps of K of one tile of 16 F x 16 F outputs and add their sums
+// ---- few tiles: the W waves of a workgroup share the steps of K of one tile of SIDE x SIDE outputs and add their sums
 // through LDS in a fixed tree.  SRC: the activations' own type, quantised by each wave for its steps, or void: packed.
 // A step's fragments are fetched one step ahead.
-template <typename T, typename SRC, int F>
-__global__ __launch_bounds__(F == 4 ? 512 : 1024) void mx_split_kernel(MxArgs a) {
+
+// one 16 x 16 tile (16x16x128: lane l holds row l % 16, k block l / 16), its fragments gathered from the units by blocks
+struct Tile16 {
+  static constexpr int SIDE = 16, NF = 1, NA = 1;      // fragments a step, accumulators (of four floats)
+  f32x4 acc[1];
+  static __device__ __forceinline__ int unit_slot(int lane, int r) {      // 16-byte slot of (row r of 64, this lane's block)
+    const int kb = lane >> 4;
+    return ((kb >> 1) * 2 + (r >> 5)) * 64 + (kb & 1) * 32 + frag_row(r & 31);
+  }
+  __device__ __forceinline__ void mma(const u32x4 (&w)[1], const u32x4 (&x)[1], uint32_t sw, uint32_t sx) {
+    acc[0] = mma16(w[0], x[0], acc[0], sw, sx);
+  }
+};
+// one 32 x 32 tile: two fragments a step
+struct Tile32 {
+  static constexpr int SIDE = 32, NF = 2, NA = 4;
+  f32x16 acc[1];
+  __device__ __forceinline__ void mma(const u32x4 (&w)[2], const u32x4 (&x)[2], uint32_t sw, uint32_t sx) {
+    acc[0] = mma32<0, 0>(w[0], x[0], acc[0], sw, sx);
+    acc[0] = mma32<1, 1>(w[1], x[1], acc[0], sw, sx);
+  }
+};
+// 64 x 64, whole units: four fragments a step
+struct Tile64 {
+  static constexpr int SIDE = 64, NF = 4, NA = 16;
+  f32x16 acc[4];      // [columns' half][rows' half]
+  __device__ __forceinline__ void mma(const u32x4 (&w)[4], const u32x4 (&x)[4], uint32_t sw, uint32_t sx) {
+    static_for<8>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, kh = i >> 2, wf = i >> 1 & 1, xf = i & 1;
+      acc[wf * 2 + xf] = mma32<kh * 2 + wf, kh * 2 + xf>(w[kh * 2 + wf], x[kh * 2 + xf], acc[wf * 2 + xf], sw, sx);
+    });
+  }
+};
+
+template <typename T, typename SRC, typename TILE>
+__global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
   typedef typename std::conditional<RAW, SRC, bf16>::type S;
+  constexpr int SIDE = TILE::SIDE, NF = TILE::NF, NA = TILE::NA;
   extern __shared__ f32x4 xch[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
-  const uint32_t ng = blockIdx.x / (4 / F), f0 = blockIdx.x % (4 / F) * F;      // weights: group of 64, first fragment in it
-  const uint32_t m0 = blockIdx.y * 16 * F;
-  const u32x4* wc = a.wc + (uint64_t)ng * a.kt * 256 + f0 * 64 + lane;
-  const uint32_t* ws = a.ws + (uint64_t)ng * a.kt * 64 + lane;
-  // row of this lane in fragment fx of the tile; the packed order where the tile is a whole group
-  auto row_of = [&](int fx) __attribute__((always_inline)) { return m0 + (F == 4 ? frag_row(fx, lane & 15) : fx * 16 + (lane & 15)); };
-  f32x4 acc[F][F];
+  const uint32_t n0 = blockIdx.x * SIDE, m0 = blockIdx.y * SIDE, ng = n0 >> 6, xg = m0 >> 6;
+  // where this lane's blocks of fragment f lie in a unit (16-byte slots), for the rows from r0 (in the unit) on
+  auto slot = [&](uint32_t r0, int f) __attribute__((always_inline)) -> int {
+    if constexpr (SIDE == 16) return Tile16::unit_slot(lane, r0 + (lane & 15));
+    else if constexpr (SIDE == 32) return (f * 2 + (r0 >> 5)) * 64 + lane;
+    else return f * 64 + lane;
+  };
+  // row and first k (in the step) of this lane's block of fragment f, for activations quantised here: in a unit's order,
+  // so that both sources give the same tile
+  auto raw_row = [&](int f) __attribute__((always_inline)) -> uint32_t {
+    if constexpr (SIDE == 16) return m0 + (lane & 15);
+    else if constexpr (SIDE == 32) return m0 + frag_row(lane & 31);
+    else return m0 + (f & 1) * 32 + frag_row(lane & 31);
+  };
+  auto raw_k = [&](int f) __attribute__((always_inline)) -> int {
+    if constexpr (SIDE == 16) return (lane >> 4) * 32;
+    else if constexpr (SIDE == 32) return f * 64 + (lane >> 5) * 32;
+    else return (f >> 1) * 64 + (lane >> 5) * 32;
+  };
+  // the scale bytes of this lane's blocks out of a unit's word(s), byte f: fragment f
+  auto scales = [&](const uint32_t* unit, uint32_t r0) __attribute__((always_inline)) -> uint32_t {
+    if constexpr (SIDE == 64) {
+      return unit[lane];
+    } else if constexpr (SIDE == 32) {
+      const uint32_t v = unit[lane] >> (8 * (r0 >> 5));      // fragments r0 / 32 and 2 + r0 / 32
+      return (v & 255u) | (v >> 8 & 0xff00u);
+    } else {
+      const int sl = slot(r0, 0);
+      return unit[sl & 63] >> (8 * (sl >> 6)) & 255u;
+    }
+  };
+  TILE t;
+  if constexpr (SIDE == 16) {
 #pragma unroll
-  for (int w = 0; w < F; ++w) {
-    const f32x4 b = wave == 0 ? bias4(a, ng * 64, f0 + w, lane) : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t n = n0 + (lane >> 4) * 4 + i;
+      t.acc[0][i] = (wave == 0 && a.bias != nullptr && n < a.N) ? a.bias[n] : 0.f;
+    }
+  } else {
 #pragma unroll
-    for (int x = 0; x < F; ++x) acc[w][x] = b;
+    for (int i = 0; i < NA / 4; ++i) {
+      t.acc[i] = bias16(a, n0 + (i >> 1) * 32, lane);
+      if (wave != 0)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t.acc[i][j] = 0.f;
+    }
   }
   struct Step {
-    u32x4 w[F], x[F];
-    RawBlock<S> raw[RAW ? F : 1];
+    u32x4 w[NF], x[NF];
+    RawBlock<S> raw[RAW ? NF : 1];
     uint32_t sw, sx;
   };
   auto fetch = [&](Step& s, uint32_t k) __attribute__((always_inline)) {
+    const uint64_t wu = (uint64_t)ng * a.kt + k, xu = (uint64_t)xg * a.kt + k;
 #pragma unroll
-    for (int f = 0; f < F; ++f) s.w[f] = wc[(uint64_t)k * 256 + f * 64];
-    s.sw = ws[(uint64_t)k * 64] >> (8 * f0);
+    for (int f = 0; f < NF; ++f) s.w[f] = a.wc[wu * 256 + slot(n0 & 63, f)];
+    s.sw = scales(a.ws + wu * 64, n0 & 63);
     s.sx = 0;
+    if constexpr (RAW) {
 #pragma unroll
-    for (int f = 0; f < F; ++f) {
-      const uint32_t row = row_of(f);
-      if constexpr (RAW) {
+      for (int f = 0; f < NF; ++f) {
+        const uint32_t row = raw_row(f);
         const bool there = row < a.M;
-        load_block<S, true>(reinterpret_cast<const S*>(a.x) + (int64_t)(there ? row : 0) * a.ldx, (int)k * 128 + (lane >> 4) * 32, a.K,
-                           there, s.raw[f]);
-      } else if (F == 4) {
-        s.x[f] = a.xc[((uint64_t)blockIdx.y * a.kt + k) * 256 + f * 64 + lane];
-        if (f == 0) s.sx = a.xs[((uint64_t)blockIdx.y * a.kt + k) * 64 + lane];
-      } else {
-        // where the packed order has this row: fragment and lane
-        const uint32_t g = row >> 6, r = row & 63, pf = (r >> 5 << 1) + (r >> 2 & 1), pl = (lane & 48) + (r >> 3 & 3) * 4 + (r & 3);
-        s.x[f] = a.xc[((uint64_t)g * a.kt + k) * 256 + pf * 64 + pl];
-        s.sx |= (a.xs[((uint64_t)g * a.kt + k) * 64 + pl] >> (8 * pf) & 255u) << (8 * f);
+        load_block<S, true>(reinterpret_cast<const S*>(a.x) + (int64_t)(there ? row : 0) * a.ldx, (int)k * 128 + raw_k(f), a.K, there,
+                            s.raw[f]);
       }
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; ++f) s.x[f] = a.xc[xu * 256 + slot(m0 & 63, f)];
+      s.sx = scales(a.xs + xu * 64, m0 & 63);
     }
   };
   Step nx;
@@ -340,171 +390,183 @@ __global__ __launch_bounds__(F == 4 ? 512 : 1024) void mx_split_kernel(MxArgs a)
     if (k < a.kt) fetch(nx, k);
     if constexpr (RAW) {
 #pragma unroll
-      for (int f = 0; f < F; ++f) s.sx |= mx_block(s.raw[f], s.x[f]) << (8 * f);
+      for (int f = 0; f < NF; ++f) s.sx |= mx_block(s.raw[f], s.x[f]) << (8 * f);
     }
-    static_for<F>([&](auto fw) __attribute__((always_inline)) {
-      static_for<F>([&](auto fx) __attribute__((always_inline)) {
-        constexpr int w = decltype(fw)::value, x = decltype(fx)::value;
-        acc[w][x] = mma4<w, x>(s.w[w], s.x[x], acc[w][x], s.sw, s.sx);
-      });
-    });
+    t.mma(s.w, s.x, s.sw, s.sx);
   }
-  for (int half = W >> 1; half >= 1; half >>= 1) {
+  auto part = [&](int i) __attribute__((always_inline)) -> f32x4 {
+    if constexpr (SIDE == 16) return t.acc[0];
+    else return f32x4{t.acc[i / 4][i % 4 * 4], t.acc[i / 4][i % 4 * 4 + 1], t.acc[i / 4][i % 4 * 4 + 2], t.acc[i / 4][i % 4 * 4 + 3]};
+  };
+  // down to four waves (two for the small tiles) by halves, then each of those sums and finishes its share of the tile
+  constexpr int FIN = SIDE == 64 ? 4 : SIDE == 32 ? 2 : 1;
+  const int left = W < FIN ? W : FIN, each = NA / left;
+  auto add = [&](int i, const f32x4& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (SIDE == 16) t.acc[0][j] += v[j];
+      else t.acc[i / 4][i % 4 * 4 + j] += v[j];
+    }
+  };
+  for (int half = W >> 1; half >= FIN; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
-      for (int i = 0; i < F * F; ++i) xch[((wave - half) * F * F + i) * 64 + lane] = acc[i / F][i % F];
+      for (int i = 0; i < NA; ++i) xch[((wave - half) * NA + i) * 64 + lane] = part(i);
     }
     __syncthreads();
     if (wave < half) {
 #pragma unroll
-      for (int i = 0; i < F * F; ++i) acc[i / F][i % F] += xch[(wave * F * F + i) * 64 + lane];
+      for (int i = 0; i < NA; ++i) add(i, xch[(wave * NA + i) * 64 + lane]);
     }
     __syncthreads();
   }
-  if (wave != 0) return;
-  const int q = lane >> 4;
-  with_epilogue(a, [&](auto act, auto vec) __attribute__((always_inline)) {
-    constexpr int ACT = decltype(act)::value;
-    constexpr bool V = decltype(vec)::value;
+  if (left > 1) {
+    if (wave < left) {
 #pragma unroll
-    for (int x = 0; x < F; ++x) {
-      const uint32_t m = row_of(x);
-      if constexpr (F == 1) {
-        // one fragment: four columns out of eight
-        const uint32_t n = ng * 64 + ((f0 >> 1) << 5) + (q << 3) + ((f0 & 1) << 2);
-        if (m < a.M) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < a.N) {
-              float y = mx_act<T, ACT>(acc[0][0][i]);
-              if (a.resid != nullptr) y += to_f32(reinterpret_cast<const T*>(a.resid)[(int64_t)m * a.ldr + n + i]);
-              reinterpret_cast<T*>(a.out)[(int64_t)m * a.ldo + n + i] = from_f32<T>(y);
-            }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < F / 2; ++j)
-          store8<T, ACT, V>(a, m, ng * 64 + (f0 >> 1) * 32 + j * 32 + q * 8, acc[2 * j][x], acc[2 * j + 1][x]);
-      }
+      for (int i = 0; i < NA; ++i) xch[(wave * NA + i) * 64 + lane] = part(i);
     }
-  });
+    __syncthreads();
+    if (wave < left) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+        if (i / each == wave) {
+          f32x4 v = xch[i * 64 + lane];
+          for (int w = 1; w < left; ++w) v += xch[(w * NA + i) * 64 + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (SIDE == 16) t.acc[0][j] = v[j];
+            else t.acc[i / 4][i % 4 * 4 + j] = v[j];
+          }
+        }
+    }
+  }
+  if constexpr (SIDE == 16) {
+    if (wave != 0) return;
+    const uint32_t m = m0 + (lane & 15), n = n0 + (lane >> 4) * 4;
+    if (m >= a.M) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) {
+        float y = a.act ? mx_act<T, true>(t.acc[0][i]) : t.acc[0][i];
+        if (a.resid != nullptr) y += to_f32(reinterpret_cast<const T*>(a.resid)[(int64_t)m * a.ldr + n + i]);
+        reinterpret_cast<T*>(a.out)[(int64_t)m * a.ldo + n + i] = from_f32<T>(y);
+      }
+  } else {
+    // parts i, i + 1 (i even): 8 columns from col8(i) on of this lane's row in half i / 4 % 2 of the rows
+    auto col8 = [&](int i) __attribute__((always_inline)) -> uint32_t { return (i >> 3) * 32 + (i & 2) * 8 + ((lane >> 5) << 3); };
+    with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NA; i += 2) {
+        if (wave >= left || i / each != wave) continue;
+        f32x16 r;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = t.acc[i / 4][(i & 2) * 4 + (j & 7)];
+        store8<T, decltype(act)::value, decltype(whole)::value, 0>(a, m0 + ((i >> 2) & 1) * 32 + frag_row(lane & 31), n0 + col8(i), r);
+      }
+    });
+  }
 }
 
-// ---- many rows, short K (KS steps of 128): a wave quantises its 64 rows once and keeps them in registers; the workgroup
-// runs over its groups of 64 columns, whose weights the next group's LDS-DMA brings while this one is multiplied and
-// written.  Bound by the write of the output and the arithmetic on it.
+// ---- many rows, short K (KS steps of 128): a workgroup of W (two to eight) waves quantises 64 rows once into LDS and its
+// waves take every W-th group of 64 columns.  The weights' fragments come straight from the caches into
+// a ring of registers, a group ahead; the rows' are read from LDS a step at a time.  Bound by the write of the output (a
+// store instruction whose lanes lie in many rows holds the CU's address path for some 100 cycles) and the arithmetic on it.
 template <typename T, typename SRC, int KS>
-__global__ __launch_bounds__(256, KS <= 2 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
+__global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
   typedef typename std::conditional<RAW, SRC, bf16>::type S;
-  constexpr int STAGE = KS * (4096 + 256);      // codes of KS steps, their scales
-  constexpr int PIECES = KS * 4 + (KS + 3) / 4, PER = (PIECES + 3) / 4;      // of 1 KB (the last may be part empty), a wave
-  __shared__ __attribute__((aligned(1024))) char st0[PIECES * 1024];
-  __shared__ __attribute__((aligned(1024))) char st1[PIECES * 1024];
-  static_assert(STAGE <= PIECES * 1024, "stage");
+  __shared__ u32x4 xl[KS][4][64];
+  __shared__ uint8_t sl[KS][64][4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups are dealt round-robin to the 8 XCDs: XCD x takes the x-th eighth of the list (rows, columns), columns
   // fastest, so that the workgroups that read the same rows do so through the same L2
   const uint32_t pos = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   const uint32_t splits = (a.ngroups + a.per - 1) / a.per;
-  const uint32_t mb = pos / splits, g0 = pos % splits * a.per;
-  if ((uint64_t)mb * 256 >= a.M) return;      // (the whole workgroup)
+  const uint32_t mg = pos / splits, g0 = pos % splits * a.per;
+  if ((uint64_t)mg * 64 >= a.M) return;      // (the whole workgroup)
   const uint32_t g1 = g0 + a.per < a.ngroups ? g0 + a.per : a.ngroups;
-  const uint32_t mg = mb * 4 + wave;
-  // pieces wave, wave + 4, ... of a group's weights; the surplus ones repeat the last, lanes past the scales' end read
-  // their first bytes again
-  auto request = [&](uint32_t g, char* st) __attribute__((always_inline)) {
+  // the ring: fragments and scales of the KS steps of this wave's next group
+  u32x4 wr[KS][4];
+  uint32_t ws[KS];
+  auto refill = [&](uint32_t g, int k) __attribute__((always_inline)) {
+    const uint64_t u = (uint64_t)(g < a.ngroups ? g : a.ngroups - 1) * KS + k;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int p = wave + 4 * i < PIECES ? wave + 4 * i : PIECES - 1;
-      if (p < KS * 4) {
-        glds16e(a.wc + ((uint64_t)g * KS * 4 + p) * 64 + lane, st + p * 1024);
-      } else {
-        const int o = (p - KS * 4) * 64 + lane;
-        glds16e(reinterpret_cast<const u32x4*>(a.ws) + (uint64_t)g * KS * 16 + (o < KS * 16 ? o : 0), st + p * 1024);
-      }
-    }
+    for (int f = 0; f < 4; ++f) wr[k][f] = a.wc[u * 256 + f * 64 + lane];
+    ws[k] = a.ws[u * 64 + lane];
   };
-  request(g0, st0);
-  u32x4 xf[KS][4];
-  uint32_t sx[KS];
-  const bool work = (uint64_t)mg * 64 < a.M;      // (a wave without rows only helps to fetch)
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
+  for (int k = 0; k < KS; ++k) refill(g0 + wave, k);
+  const int W = blockDim.x >> 6;
+#pragma unroll 1
+  for (int f = wave; f < 4; f += W) {
+    const uint32_t row = mg * 64 + (f & 1) * 32 + frag_row(lane & 31);
     if constexpr (RAW) {
-      // (a step, or in fp32 half a step, at a time: more in flight costs more registers than the multiplication has)
-      constexpr int FB = sizeof(S) == 2 ? 4 : 2;
-      sx[k] = 0;
+      constexpr int KB = sizeof(S) == 2 ? 3 : 2;      // blocks in flight at a time
 #pragma unroll
-      for (int f0 = 0; f0 < 4; f0 += FB) {
-        RawBlock<S> r[FB];
+      for (int k0 = 0; k0 < KS; k0 += KB) {
+        RawBlock<S> r[KB];
 #pragma unroll
-        for (int f = 0; f < FB; ++f) {
-          const uint32_t row = mg * 64 + frag_row(f0 + f, lane & 15);
-          load_block<S, true>(reinterpret_cast<const S*>(a.x) + (int64_t)(row < a.M ? row : 0) * a.ldx, k * 128 + (lane >> 4) * 32,
-                              a.K, row < a.M, r[f]);
-        }
+        for (int k = 0; k < KB; ++k)
+          if (k0 + k < KS)
+            load_block<S, true>(reinterpret_cast<const S*>(a.x) + (int64_t)(row < a.M ? row : 0) * a.ldx,
+                                (k0 + k) * 128 + (f >> 1) * 64 + (lane >> 5) * 32, a.K, row < a.M, r[k]);
 #pragma unroll
-        for (int f = 0; f < FB; ++f) {
-          sx[k] |= mx_block(r[f], xf[k][f0 + f]) << (8 * (f0 + f));
-          asm volatile("" : "+v"(xf[k][f0 + f]) : : "memory");
-        }
+        for (int k = 0; k < KB; ++k)
+          if (k0 + k < KS) {
+            u32x4 c;
+            sl[k0 + k][lane][f] = (uint8_t)mx_block(r[k], c);
+            xl[k0 + k][f][lane] = c;
+          }
       }
     } else {
-      const uint32_t g = work ? mg : 0;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) xf[k][f] = a.xc[((uint64_t)g * KS + k) * 256 + f * 64 + lane];
-      sx[k] = a.xs[((uint64_t)g * KS + k) * 64 + lane];
+      for (int k = 0; k < KS; ++k) {
+        const uint64_t u = (uint64_t)mg * KS + k;
+        xl[k][f][lane] = a.xc[u * 256 + f * 64 + lane];
+        if (f == 0) *reinterpret_cast<uint32_t*>(&sl[k][lane][0]) = a.xs[u * 64 + lane];
+      }
     }
   }
-  auto group = [&](uint32_t g, const char* st, char* other) __attribute__((always_inline)) {
-    // this group's weights have landed for every wave, and everyone is done with the other stage
-    wait_vm_then_barrier<0, true>();
-    if (g + 1 < g1) request(g + 1, other);
-    if (!work) return;
-    f32x4 acc[4][4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const f32x4 b = bias4(a, g * 64, w, lane);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) acc[w][x] = b;
-    }
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t g = g0 + wave; g < g1; g += W) {
+    Tile64 t;
+    t.acc[0] = t.acc[1] = bias16(a, g * 64, lane);
+    t.acc[2] = t.acc[3] = bias16(a, g * 64 + 32, lane);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      u32x4 wf[4];
-#pragma unroll
-      for (int f = 0; f < 4; ++f) wf[f] = *reinterpret_cast<const u32x4*>(st + (k * 4 + f) * 1024 + lane * 16);
-      const uint32_t sw = *reinterpret_cast<const uint32_t*>(st + KS * 4096 + k * 256 + lane * 4);
-      static_for<4>([&](auto fw) __attribute__((always_inline)) {
-        static_for<4>([&](auto fx) __attribute__((always_inline)) {
-          constexpr int w = decltype(fw)::value, x = decltype(fx)::value;
-          acc[w][x] = mma4<w, x>(wf[w], xf[k][x], acc[w][x], sw, sx[k]);
-        });
-      });
+      const u32x4 xf[4] = {xl[k][0][lane], xl[k][1][lane], xl[k][2][lane], xl[k][3][lane]};
+      t.mma(wr[k], xf, ws[k], *reinterpret_cast<const uint32_t*>(&sl[k][lane][0]));
+      refill(g + W, k);
     }
-    // (opaque: the compiler would otherwise move the multiplications in front of each row's store and keep every weight
-    // fragment of the group for them)
+    // (opaque: the compiler would otherwise move the multiplications in front of each row's store)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(acc[i / 4][i % 4]));
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(t.acc[i]));
     with_epilogue(a, [&](auto act, auto vec) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const uint32_t m = mg * 64 + frag_row(x, lane & 15), n = g * 64 + (lane >> 4) * 8;
-        store8<T, decltype(act)::value, decltype(vec)::value>(a, m, n, acc[0][x], acc[1][x]);
-        store8<T, decltype(act)::value, decltype(vec)::value>(a, m, n + 32, acc[2][x], acc[3][x]);
-      }
+      for (int i = 0; i < 4; ++i)
+        store_tile<T, decltype(act)::value, decltype(vec)::value>(a, mg * 64 + (i & 1) * 32 + frag_row(lane & 31),
+                                                                  g * 64 + (i >> 1) * 32, lane, t.acc[i]);
     });
-  };
-#pragma unroll 1
-  for (uint32_t g = g0; g < g1; g += 2) {
-    group(g, st0, st1);
-    if (g + 1 < g1) group(g + 1, st1, st0);
   }
 }
 
 // ---- large products: 256 x 256 outputs a workgroup, 128 x 128 a wave, so that a byte read from LDS meets 128 others.
 // Four LDS stages of a step (128 k) each, filled by LDS-DMA: while step s multiplies from registers, the fragments of step
 // s + 1 are read from their stage between the multiplications, stage s + 2 is landing and s + 3 is requested.
+// LDS-DMA of 16 bytes a lane as an instruction of its own.  Through the builtin the compiler follows which transfers may
+// still be filling which array, loses track at the loop's end and waits for all of them there, the newest included; here
+// it knows of none, and the kernel's own counted waits are the only ones.  (No register is written; the address registers
+// are read when the instruction issues.)
+__device__ __forceinline__ void dma16(const void* src, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
 constexpr int LG_STAGE = 2 * (16 * 1024 + 1024);      // codes of 256 rows and 256 columns, their scales
 
 template <typename T>
@@ -548,12 +610,15 @@ __global__ __launch_bounds__(256, 1) void mx_large_kernel(MxArgs a) {
       ssrc = reinterpret_cast<const u32x4*>(a.ws) + (uint64_t)gg * a.kt * 16 + (lane & 15);
     }
   }
+  // request p (of nine) of step k's data into a stage
+  auto request1 = [&](uint32_t k, uint32_t base, int p) __attribute__((always_inline)) {
+    if (p < 8) dma16(src[p / 4] + (uint64_t)k * 256 + (p % 4) * 64, base + (wave * 8 + p) * 1024);
+    else dma16(ssrc + (uint64_t)k * 16, base + 32 * 1024 + (wave & 1) * 1024);
+  };
   auto request = [&](uint32_t k, char* st) __attribute__((always_inline)) {
+    const uint32_t base = __builtin_amdgcn_readfirstlane(lds_address(st));
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int f = 0; f < 4; ++f) glds16e(src[i] + (uint64_t)k * 256 + f * 64, st + (wave * 8 + i * 4 + f) * 1024);
-    glds16e(ssrc + (uint64_t)k * 16, st + 32 * 1024 + (wave & 1) * 1024);
+    for (int p = 0; p < 9; ++p) request1(k, base, p);
   };
   struct Frags {
     u32x4 x[8], w[8];
@@ -568,40 +633,53 @@ __global__ __launch_bounds__(256, 1) void mx_large_kernel(MxArgs a) {
       f.sw[i / 4] = *reinterpret_cast<const uint32_t*>(st + 33 * 1024 + (wn * 2 + i / 4) * 256 + lane * 4);
     }
   };
-  f32x4 acc[8][8];      // [weights' fragment][activations' fragment]
+  f32x16 acc[4][4];      // [32 columns][32 rows]
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const f32x4 b = bias4(a, nt * 256 + wn * 128 + (w >> 2) * 64, w & 3, lane);
+  for (int w = 0; w < 4; ++w) {
+    const f32x16 b = bias16(a, nt * 256 + wn * 128 + w * 32, lane);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
+    for (int x = 0; x < 4; ++x) {
       acc[w][x] = b;
       asm volatile("" : "+a"(acc[w][x]));
     }
   }
   const uint32_t kt = a.kt;
   char* const stages[4] = {st0, st1, st2, st3};
+  // (in this order: the waits count requests)
   request(0, st0);
   request(1 < kt ? 1 : 0, st1);
   request(2 < kt ? 2 : 0, st2);
   wait_vm_then_barrier<18, false>();
 #pragma unroll
   for (int i = 0; i < 8; ++i) read1(fr[0], st0, i);
-  // step s (s % 4 == P): nine requests of step s + 2 may be out, those of s + 1 have landed.  Steps past the end repeat
+  wait_vm_then_barrier<9, true>();
+  // step s (s % 4 == P): when it begins, those of step s + 1 have landed for every wave and the nine of s + 2 may be out.  Steps past the end repeat
   // the last one's requests, so that the count holds.
   auto step = [&](uint32_t s, auto pc) __attribute__((always_inline)) {
     constexpr int P = decltype(pc)::value;
-    wait_vm_then_barrier<9, true>();
-    request(s + 3 < kt ? s + 3 : kt - 1, stages[(P + 3) & 3]);
+    const uint32_t later = s + 3 < kt ? s + 3 : kt - 1, base = __builtin_amdgcn_readfirstlane(lds_address(stages[(P + 3) & 3]));
     Frags& cur = fr[P & 1];
     Frags& nxt = fr[(P & 1) ^ 1];
+    // fragment i of an operand: rows 64 (i / 4) + 32 (i % 2) + ... of the wave's 128, half i / 2 % 2 of the step's k
     static_for<8>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int x = decltype(ic)::value;
-      read1(nxt, stages[(P + 1) & 3], x);
-      static_for<8>([&](auto wc) __attribute__((always_inline)) {
-        constexpr int w = decltype(wc)::value;
-        acc[w][x] = mma4<w % 4, x % 4>(cur.w[w], cur.x[x], acc[w][x], cur.sw[w / 4], cur.sx[x / 4]);
+      constexpr int i = decltype(ic)::value, kh = i >> 2, xr = i & 3, xi = (xr >> 1) * 4 + kh * 2 + (xr & 1);
+      // (a request occupies the CU's address path for some 33 cycles and holds up what its wave issues behind it: one at
+      // a time between the multiplications, not nine in front of them)
+      request1(later, base, i);
+      if (i == 7) request1(later, base, 8);
+      read1(nxt, stages[(P + 1) & 3], i);
+      static_for<4>([&](auto wc) __attribute__((always_inline)) {
+        constexpr int wr = decltype(wc)::value, wi = (wr >> 1) * 4 + kh * 2 + (wr & 1);
+        acc[wr][xr] = mma32<wi % 4, xi % 4>(cur.w[wi], cur.x[xi], acc[wr][xr], cur.sw[wi / 4], cur.sx[xi / 4]);
       });
+      __builtin_amdgcn_sched_barrier(0);
     });
+    // (the reads belong to this step: the compiler would otherwise move each in front of its use, one step later, and
+    // wait there)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(nxt.x[i]), "+v"(nxt.w[i]));
+    asm volatile("" : "+v"(nxt.sx[0]), "+v"(nxt.sx[1]), "+v"(nxt.sw[0]), "+v"(nxt.sw[1]));
+    wait_vm_then_barrier<9, true>();
   };
   // (one loop left from four places, the accumulators pinned where the multiplications update them in place: with the
   // last steps behind the loop the compiler shuffles and spills all 256 of them between the two)
@@ -620,16 +698,14 @@ __global__ __launch_bounds__(256, 1) void mx_large_kernel(MxArgs a) {
   }
   wait_vm_then_barrier<0, true>();      // nothing of this workgroup writes LDS after its end
 #pragma unroll
-  for (int i = 0; i < 64; ++i) asm volatile("" : "+a"(acc[i / 8][i % 8]));
+  for (int i = 0; i < 16; ++i) asm volatile("" : "+a"(acc[i / 4][i % 4]));
   with_epilogue(a, [&](auto act, auto vec) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const uint32_t m = mt * 256 + wm * 128 + (x >> 2) * 64 + frag_row(x & 3, lane & 15);
-      const uint32_t n = nt * 256 + wn * 128 + (lane >> 4) * 8;
+    for (int x = 0; x < 4; ++x)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        store8<T, decltype(act)::value, decltype(vec)::value>(a, m, n + j * 32, acc[2 * j][x], acc[2 * j + 1][x]);
-    }
+      for (int w = 0; w < 4; ++w)
+        store_tile<T, decltype(act)::value, decltype(vec)::value>(a, mt * 256 + wm * 128 + x * 32 + frag_row(lane & 31),
+                                                                  nt * 256 + wn * 128 + w * 32, lane, acc[w][x]);
   });
 }
 
@@ -644,7 +720,7 @@ int check_mx(const char* who, int64_t rows, int64_t K, int dtype) {
   UNETK_CHECK_ARG(dtype == UNETK_F32 || dtype == UNETK_BF16, "%s: unsupported dtype %d", who, dtype);
   UNETK_CHECK_ARG(rows >= 1 && rows <= MX_MAX_ROWS && K >= 1 && K <= MX_MAX_K, "%s: a %lld x %lld matrix", who,
                   (long long)rows, (long long)K);
-  UNETK_CHECK_ARG(units_of(rows, (int)K) < (int64_t)1 << 26, "%s: a %lld x %lld matrix", who, (long long)rows, (long long)K);
+  UNETK_CHECK_ARG(units_of(rows, (int)K) < (int64_t)1 << 24, "%s: a %lld x %lld matrix", who, (long long)rows, (long long)K);
   return UNETK_OK;
 }
 
@@ -657,37 +733,51 @@ Plan plan_of(int64_t M, int64_t K, int64_t N) {
   return SPLIT;
 }
 
-template <typename T, typename SRC, int F> void launch_split(const MxArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)cdiv(a.N, 64) * (4 / F), (unsigned)cdiv(a.M, 16 * F));
+template <typename T, typename SRC, typename TILE> void launch_split(const MxArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(a.N, TILE::SIDE), (unsigned)cdiv(a.M, TILE::SIDE));
   // waves a tile: about 4096 in all, at least a step each
   const int64_t tiles = (int64_t)grid.x * grid.y;
   int W = 1;
-  while (W < (F == 4 ? 8 : 16) && tiles * W < 4096 && (uint32_t)W * 2 <= a.kt) W *= 2;
-  hipLaunchKernelGGL((mx_split_kernel<T, SRC, F>), grid, dim3(64 * W), W / 2 * F * F * 1024, stream, a);
+  while (W < (TILE::SIDE == 64 ? 8 : 16) && tiles * W < 4096 && (uint32_t)W * 2 <= a.kt) W *= 2;
+  const int fin = TILE::SIDE == 64 ? 4 : TILE::SIDE == 32 ? 2 : 1, parts = W / 2 > fin ? W / 2 : W < fin ? W : fin;
+  hipLaunchKernelGGL((mx_split_kernel<T, SRC, TILE>), grid, dim3(64 * W), W > 1 ? parts * TILE::NA * 1024 : 0, stream, a);
 }
 template <typename T, typename SRC> void launch_split_f(const MxArgs& a, hipStream_t stream) {
-  if (a.M <= 16) launch_split<T, SRC, 1>(a, stream);
+  if (a.M <= 16) launch_split<T, SRC, Tile16>(a, stream);
   else if constexpr (std::is_same<SRC, float>::value) return;      // (never asked for: unetk_mx_linear_x_supported)
-  else if (a.M <= 32) launch_split<T, SRC, 2>(a, stream);
-  else launch_split<T, SRC, 4>(a, stream);
+  else if (a.M <= 32) launch_split<T, SRC, Tile32>(a, stream);
+  else launch_split<T, SRC, Tile64>(a, stream);
 }
 
 template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stream) {
   a.ngroups = (uint32_t)cdiv(a.N, 64);
-  const uint32_t blocks = (uint32_t)cdiv(a.M, 256);
-  // the columns are split until there are workgroups enough for the chip
-  uint32_t splits = 1;
-  while (blocks * splits < 512 && splits < a.ngroups) ++splits;
+  const uint32_t blocks = (uint32_t)cdiv(a.M, 64);
+  // How many waves share 64 rows, and over how many workgroups their columns are split, from what bounds the kernel, in
+  // cycles of a CU: its address path (about 100 for a load or store whose lanes lie in many rows: 16 of a step's rows, 8 of a
+  // group's results; 33 for 1 KB of weights), and the rounds of resident workgroups times a wave's own way through its
+  // share.  (16384 x 384 -> 1152: 14.9 us with six waves and one split, 20.4 with four and three, 25.9 with three and six.)
+  const double ks = a.kt, resident = 256.0 * (a.kt == 1 ? 16 : a.kt <= 3 ? 12 : 8);
+  uint32_t W = 4, splits = 1;
+  double best = 1e30;
+  for (uint32_t s = 1; s <= 16 && s <= a.ngroups; ++s)
+    for (uint32_t w = 2; w <= 8; ++w) {
+      const uint32_t per = (a.ngroups + s - 1) / s, used = (a.ngroups + per - 1) / per;
+      const double path = blocks * (used * ks * 1600.0 + a.ngroups * (800.0 + ks * 140.0)) / 256.0;
+      const double rounds = (double)blocks * used * w / resident;
+      const double way = ((4 + w - 1) / w) * (1500.0 + ks * 500.0) + ((per + w - 1) / w) * (1800.0 + ks * 400.0);
+      const double waves = (rounds > 1.0 ? rounds : 1.0) * way, cost = (path > waves ? path : waves) + 0.2 * (path + waves);
+      if (cost < best) best = cost, W = w, splits = s;
+    }
   a.per = (a.ngroups + splits - 1) / splits;
   splits = (a.ngroups + a.per - 1) / a.per;
-  const dim3 grid((blocks * splits + 7) / 8 * 8);
+  const dim3 grid((blocks * splits + 7) / 8 * 8), threads(64 * W);
   switch (a.kt) {
-    case 1: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 1>), grid, dim3(256), 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 2>), grid, dim3(256), 0, stream, a); break;
-    case 3: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 3>), grid, dim3(256), 0, stream, a); break;
-    case 4: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 4>), grid, dim3(256), 0, stream, a); break;
-    case 5: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 5>), grid, dim3(256), 0, stream, a); break;
-    default: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 6>), grid, dim3(256), 0, stream, a); break;
+    case 1: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 1>), grid, threads, 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 2>), grid, threads, 0, stream, a); break;
+    case 3: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 3>), grid, threads, 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 4>), grid, threads, 0, stream, a); break;
+    case 5: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 5>), grid, threads, 0, stream, a); break;
+    default: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 6>), grid, threads, 0, stream, a); break;
   }
 }
 
@@ -713,7 +803,7 @@ int mx_linear_impl(const void* x, int64_t ldx, const void* xcodes, const void* x
   UNETK_CHECK_ARG(wcodes && wscales && out && ldo >= N && (resid == nullptr || ldr >= N),
                   "mx_linear: null operand or overlapping rows");
   UNETK_CHECK_ARG(aligned16(wcodes) && aligned16(wscales), "mx_linear: misaligned packed operand");
-  UNETK_CHECK_ARG(act >= 0 && act <= 2, "mx_linear: activation %d", act);
+  UNETK_CHECK_ARG(act == 0 || act == 2, "mx_linear: activation %d", act);
   // (grids: one block axis per 16 columns, one per 16...64 rows)
   UNETK_CHECK_ARG(N <= (int64_t)1 << 24 && (M <= (int64_t)1 << 21 || plan_of(M, K, N) != SPLIT), "mx_linear: %lld x %lld outputs",
                   (long long)M, (long long)N);
@@ -722,8 +812,7 @@ int mx_linear_impl(const void* x, int64_t ldx, const void* xcodes, const void* x
   a.xc = (const u32x4*)xcodes; a.xs = (const uint32_t*)xscales; a.wc = (const u32x4*)wcodes; a.ws = (const uint32_t*)wscales;
   a.out = out; a.bias = bias; a.resid = resid; a.ldo = ldo; a.ldr = ldr; a.M = (uint32_t)M; a.N = (uint32_t)N;
   a.kt = (uint32_t)((K + 127) / 128); a.K = (int)K; a.act = act;
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  a.vec = N % E == 0 && ldo % E == 0 && aligned16(out) && (!resid || (ldr % E == 0 && aligned16(resid)));
+  a.whole = N % (dtype == UNETK_BF16 ? 8 : 4) == 0;
   const Plan plan = plan_of(M, K, N);
   if (dtype == UNETK_BF16) launch_mx<bf16>(a, plan, stream);
   else launch_mx<float>(a, plan, stream);
@@ -750,16 +839,15 @@ int unetk_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int d
   const uint32_t kt = (uint32_t)((K + 127) / 128);
   const uint64_t units = (uint64_t)units_of(rows, (int)K);
   const dim3 grid((unsigned)((units + 3) / 4));
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  const bool vec = K % E == 0 && ldx % E == 0 && aligned16(x);
+  const bool whole = K % (dtype == UNETK_BF16 ? 8 : 4) == 0;
 #define MX_QUANT(T, V)                                                                                                \
   hipLaunchKernelGGL((mx_quantize_kernel<T, V>), grid, dim3(256), 0, stream, (const T*)x, ldx, (uint32_t)rows, (int)K, kt, \
                      units, (u32x4*)codes, (uint32_t*)scales)
   if (dtype == UNETK_BF16) {
-    if (vec) MX_QUANT(bf16, true);
+    if (whole) MX_QUANT(bf16, true);
     else MX_QUANT(bf16, false);
   } else {
-    if (vec) MX_QUANT(float, true);
+    if (whole) MX_QUANT(float, true);
     else MX_QUANT(float, false);
   }
 #undef MX_QUANT
@@ -774,16 +862,19 @@ int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
   UNETK_CHECK_ARG(out && codes && scales && ldo >= K && aligned16(codes) && aligned16(scales),
                   "mx_dequantize: null or misaligned operand, or overlapping rows");
   const uint32_t kt = (uint32_t)((K + 127) / 128);
-  const uint64_t units = (uint64_t)units_of(rows, (int)K);
-  const dim3 grid((unsigned)((units + 3) / 4));
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  const int vec = K % E == 0 && ldo % E == 0 && aligned16(out);
-  if (dtype == UNETK_BF16)
-    hipLaunchKernelGGL(mx_dequantize_kernel<bf16>, grid, dim3(256), 0, stream, (const u32x4*)codes, (const uint32_t*)scales,
-                       (uint32_t)rows, (int)K, kt, units, (bf16*)out, ldo, vec);
-  else
-    hipLaunchKernelGGL(mx_dequantize_kernel<float>, grid, dim3(256), 0, stream, (const u32x4*)codes, (const uint32_t*)scales,
-                       (uint32_t)rows, (int)K, kt, units, (float*)out, ldo, vec);
+  const dim3 grid((unsigned)units_of(rows, (int)K));
+  const bool whole = K % (dtype == UNETK_BF16 ? 8 : 4) == 0;
+#define MX_DEQUANT(T, V)                                                                                              \
+  hipLaunchKernelGGL((mx_dequantize_kernel<T, V>), grid, dim3(256), 0, stream, (const u32x4*)codes, (const uint32_t*)scales, \
+                     (uint32_t)rows, (int)K, kt, (T*)out, ldo)
+  if (dtype == UNETK_BF16) {
+    if (whole) MX_DEQUANT(bf16, true);
+    else MX_DEQUANT(bf16, false);
+  } else {
+    if (whole) MX_DEQUANT(float, true);
+    else MX_DEQUANT(float, false);
+  }
+#undef MX_DEQUANT
   UNETK_CHECK_LAUNCH();
   return UNETK_OK;
 }
@@ -799,8 +890,7 @@ int unetk_mx_linear_x_supported(int64_t M, int64_t K, int64_t N, int dtype) {
 int unetk_mx_linear_x(const void* x, int64_t ldx, const void* wcodes, const void* wscales, void* out, int64_t ldo, int64_t M,
                       int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
                       hipStream_t stream) {
-  const int E = dtype == UNETK_BF16 ? 8 : 4;
-  UNETK_CHECK_ARG(x && ldx >= K && ldx % E == 0 && aligned16(x), "mx_linear_x: null or unaligned activations");
+  UNETK_CHECK_ARG(x && ldx >= K, "mx_linear_x: null activations or overlapping rows");
   UNETK_CHECK_ARG(unetk_mx_linear_x_supported(M, K, N, dtype), "mx_linear_x: %lld x %lld x %lld is quantised first", (long long)M,
                   (long long)K, (long long)N);
   return mx_linear_impl(x, ldx, nullptr, nullptr, wcodes, wscales, out, ldo, M, K, N, bias, act, resid, ldr, dtype, stream);

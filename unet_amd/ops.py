@@ -1171,7 +1171,7 @@ def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
 def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None):
     """act(x @ w^T + bias) + resid with both operands in microscaled 4 bits and fp32 sums; for prediction (it has no
     gradient).  x (..., K): a float32 or bfloat16 tensor, quantised on the way, or an MxTensor (quantised once for
-    several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none, 1 ReLU, 2 GELU (erf form);
+    several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none, 2 GELU (erf form);
     resid: (..., N) of the result's type.  The result has x's type (``dtype`` for an MxTensor, bfloat16 if not given); out:
     a (..., N) tensor or channel slice to write it to."""
     if not isinstance(w, MxTensor) or len(w.shape) != 2:
@@ -1184,8 +1184,8 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
         raise ValueError(f"mx_linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
     if x.device != w.device:
         raise ValueError(f"mx_linear: x on {x.device}, w on {w.device}")
-    if act not in (0, 1, 2):
-        raise ValueError(f"mx_linear: act {act!r} (0 none, 1 ReLU, 2 GELU)")
+    if act not in (0, 2):
+        raise ValueError(f"mx_linear: act {act!r} (0 none, 2 GELU)")
     if quantised:
         dt, rows = dtype or torch.bfloat16, x.rows
     else:
@@ -1208,8 +1208,7 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
             out = torch.empty(shape, dtype=dt, device=dev)
         if rows and N:
             lib = _lib.load()
-            if not quantised and ldx * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0 and \
-                    lib.unetk_mx_linear_x_supported(rows, K, N, code):
+            if not quantised and lib.unetk_mx_linear_x_supported(rows, K, N, code):
                 call("unetk_mx_linear_x", x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, rows,
                      K, N, bias, act, _at(resid), ldr, code, stream())
             else:
