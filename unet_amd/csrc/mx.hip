@@ -128,28 +128,36 @@ __device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
   return (code & 8u) ? -v : v;
 }
 
-// One wave: one fragment (32 rows x 64 k).  Bound by the write of the values.
+// One workgroup a unit; a lane makes 8 consecutive values, 16 lanes the 128 of a row: runs of 256 bytes (bf16) a row.  Bound
+// by the write of the values.
 template <typename T, bool WHOLE>
-__global__ __launch_bounds__(256) void mx_dequantize_kernel(const u32x4* __restrict__ codes, const uint32_t* __restrict__ scales,
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             uint32_t rows, int K, uint32_t kt, T* __restrict__ out, int64_t ldo) {
   constexpr int E = Vec16<T>::N;
   const uint64_t unit = blockIdx.x;
-  const int lane = threadIdx.x & 63, f = threadIdx.x >> 6;
-  const uint32_t row = (uint32_t)(unit / kt) * 64 + (f & 1) * 32 + frag_row(lane & 31);
-  const int k0 = (int)(unit % kt) * 128 + (f >> 1) * 64 + (lane >> 5) * 32;
-  if (row >= rows) return;
-  const u32x4 c = codes[(unit * 4 + f) * 64 + lane];
-  const uint32_t sc = scales[unit * 64 + lane] >> (8 * f) & 255u;
-  T* o = out + (int64_t)row * ldo + k0;
+  const int k8 = threadIdx.x & 15, kb = k8 >> 2;      // which 8 values of the row, in which block
+  const int k0 = (int)(unit % kt) * 128 + k8 * 8;
+  if (k0 >= K) return;
+  uint32_t c[4], sc[4];
 #pragma unroll
-  for (int j = 0; j < 32 / E; ++j) {
-    Vec16<T> v;
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 16 + (threadIdx.x >> 4);      // row of the unit
+    const int f = (kb >> 1) * 2 + (r >> 5), slot = (kb & 1) * 32 + frag_row(r & 31);
+    c[i] = codes[((unit * 4 + f) * 64 + slot) * 4 + (k8 & 3)];
+    sc[i] = scales[(unit * 64 + slot) * 4 + f];
+  }
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = j * E + e;
-      v.v[e] = from_f32<T>(mx_value(c[i / 8] >> (4 * (i % 8)), sc));
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t row = (uint32_t)(unit / kt) * 64 + i * 16 + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    T* o = out + (int64_t)row * ldo + k0;
+#pragma unroll
+    for (int j = 0; j < 8 / E; ++j) {
+      Vec16<T> v;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v.v[e] = from_f32<T>(mx_value(c[i] >> (4 * (j * E + e)), sc[i]));
+      store_part<WHOLE>(o + j * E, v, K - (k0 + j * E));
     }
-    store_part<WHOLE>(o + j * E, v, K - (k0 + j * E));
   }
 }
 
@@ -755,7 +763,7 @@ template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stre
   // How many waves share 64 rows, and over how many workgroups their columns are split, from what bounds the kernel, in
   // cycles of a CU: its address path (about 100 for a load or store whose lanes lie in many rows: 16 of a step's rows, 8 of a
   // group's results; 33 for 1 KB of weights), and the rounds of resident workgroups times a wave's own way through its
-  // share.  (16384 x 384 -> 1152: 14.9 us with six waves and one split, 20.4 with four and three, 25.9 with three and six.)
+  // share.  (16384 x 384 -> 1152: 20.2 us as picked here, 25.9 with three waves and six splits, which has the fewer rounds.)
   const double ks = a.kt, resident = 256.0 * (a.kt == 1 ? 16 : a.kt <= 3 ? 12 : 8);
   uint32_t W = 4, splits = 1;
   double best = 1e30;
@@ -865,7 +873,7 @@ int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
   const dim3 grid((unsigned)units_of(rows, (int)K));
   const bool whole = K % (dtype == UNETK_BF16 ? 8 : 4) == 0;
 #define MX_DEQUANT(T, V)                                                                                              \
-  hipLaunchKernelGGL((mx_dequantize_kernel<T, V>), grid, dim3(256), 0, stream, (const u32x4*)codes, (const uint32_t*)scales, \
+  hipLaunchKernelGGL((mx_dequantize_kernel<T, V>), grid, dim3(256), 0, stream, (const uint32_t*)codes, (const uint8_t*)scales, \
                      (uint32_t)rows, (int)K, kt, (T*)out, ldo)
   if (dtype == UNETK_BF16) {
     if (whole) MX_DEQUANT(bf16, true);

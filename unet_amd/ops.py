@@ -994,22 +994,10 @@ def _norm_pair(p, what, C, device):
     return _vector(w, what, C, device), _vector(b, what, C, device)
 
 
-class _OnDevice:
-    """Makes device ``index`` the current one for a block; nothing where it is that already (the usual case: torch's own
-    context manager costs the host 3 us)."""
-    __slots__ = ("index", "back")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.back = torch._C._cuda_getDevice()
-        if self.index != self.back:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index != self.back:
-            torch.cuda.set_device(self.back)
+def _raw_device():
+    """Index of the current device (torch's own context manager costs the host 3 us: it is entered only where this is
+    another one)."""
+    return torch._C._cuda_getDevice()
 
 
 def _at(t):
@@ -1052,14 +1040,17 @@ def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=Non
     the mean).  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
     float32.  Returns (r, n, stats): r and n dense, n None without pre; stats is what gated_norm_bwd reads (None unless
     want_stats).  n is taken from the unrounded r."""
+    a_keep = keep
     M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
-    with _OnDevice(dev):
-        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        n = torch.empty_like(r) if pw is not None else None
-        stats = torch.empty((M, 4), dtype=torch.float32, device=x.device) if want_stats else None
-        if M:
-            call("unetk_gated_norm_fwd", x.data_ptr(), ldx, f.data_ptr(), ldf, g, keep, rps, res_scale, qw, qb, pw, pb,
-                 kind == "rms", eps, r.data_ptr(), _at(n), _at(stats), M, C, code, stream())
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return gated_norm_fwd(x, f, gate, a_keep, res_scale, post, pre, kind, eps, want_stats)
+    r = torch.empty_like(x, memory_format=torch.contiguous_format)
+    n = torch.empty_like(r) if pw is not None else None
+    stats = torch.empty((M, 4), dtype=torch.float32, device=x.device) if want_stats else None
+    if M:
+        call("unetk_gated_norm_fwd", x.data_ptr(), ldx, f.data_ptr(), ldf, g, keep, rps, res_scale, qw, qb, pw, pb,
+             kind == "rms", eps, r.data_ptr(), _at(n), _at(stats), M, C, code, stream())
     return r, n, stats
 
 
@@ -1078,6 +1069,7 @@ def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, pos
     """Gradients of gated_norm_fwd (the same arguments, and its stats) from dr and dn, the gradients of r and n.  dr may
     be None where nothing else reads r; dn is given exactly when pre is.  Sums over rows are taken in a fixed order: the
     same bits every time."""
+    a_keep = keep
     M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
     if (dn is None) != (pw is None) or (dr is None and dn is None):
         raise ValueError("gated_norm_bwd: dn goes with pre, and one of dr and dn has to be there")
@@ -1092,23 +1084,25 @@ def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, pos
     if not isinstance(stats, torch.Tensor) or stats.shape != (M, 4) or stats.dtype is not torch.float32 or \
             not stats.is_cuda or stats.get_device() != dev or not stats.is_contiguous() or stats.data_ptr() % 16:
         raise ValueError(f"stats: expected what gated_norm_fwd returned for these {M} rows")
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return gated_norm_bwd(dr, dn, x, f, stats, gate, a_keep, res_scale, post, pre, kind, eps)
     device = x.device
-    with _OnDevice(dev):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-        df = torch.empty_like(dx)
-        # one block for the parameters' gradients: pre weight, pre bias, gate, post weight, post bias
-        there = (pw, pb, g, qw, qb)
-        block = torch.empty((sum(p is not None for p in there), C), dtype=torch.float32, device=device)
-        rows = iter(block.unbind(0))
-        dpw, dpb, dg, dqw, dqb = (None if p is None else next(rows) for p in there)
-        if M:
-            lib = _lib.load()
-            partials = torch.empty(lib.unetk_gated_norm_bwd_rows(M, C) * 4 * C, dtype=torch.float32, device=device)
-            call("unetk_gated_norm_bwd", _at(dr), lddr, _at(dn), lddn, x.data_ptr(), ldx, f.data_ptr(), ldf, stats.data_ptr(),
-                 g, keep, rps, res_scale, qw, qb, pw, kind == "rms", dx.data_ptr(), df.data_ptr(), _at(dg), _at(dqw),
-                 _at(dqb), _at(dpw), _at(dpb), partials.data_ptr(), M, C, code, stream())
-        else:
-            block.zero_()
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    df = torch.empty_like(dx)
+    # one block for the parameters' gradients: pre weight, pre bias, gate, post weight, post bias
+    there = (pw, pb, g, qw, qb)
+    block = torch.empty((sum(p is not None for p in there), C), dtype=torch.float32, device=device)
+    rows = iter(block.unbind(0))
+    dpw, dpb, dg, dqw, dqb = (None if p is None else next(rows) for p in there)
+    if M:
+        lib = _lib.load()
+        partials = torch.empty(lib.unetk_gated_norm_bwd_rows(M, C) * 4 * C, dtype=torch.float32, device=device)
+        call("unetk_gated_norm_bwd", _at(dr), lddr, _at(dn), lddn, x.data_ptr(), ldx, f.data_ptr(), ldf, stats.data_ptr(),
+             g, keep, rps, res_scale, qw, qb, pw, kind == "rms", dx.data_ptr(), df.data_ptr(), _at(dg), _at(dqw),
+             _at(dqb), _at(dpw), _at(dpb), partials.data_ptr(), M, C, code, stream())
+    else:
+        block.zero_()
     return GatedNormGrads(dx, df, dg, dqw, dqb, dpw, dpb)
 
 
@@ -1116,21 +1110,15 @@ class MxTensor:
     """A (..., K) tensor in microscaled 4-bit floating point (OCP MXFP4): blocks of 32 along K, E2M1 elements and one
     power-of-two scale a block, in the order in which the matrix instruction reads them.  Made by mx_quantize; read by
     mx_linear (activations or weights alike) and mx_dequantize."""
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("codes", "scales", "shape", "rows", "device", "index", "_fused")
 
     def __init__(self, codes, scales, shape):
         self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def rows(self):
-        n = 1
+        self.device, self.index = codes.device, codes.get_device()
+        self.rows = 1
         for v in self.shape[:-1]:
-            n *= v
-        return n
+            self.rows *= v
+        self._fused = {}        # as a weight: (rows, type) -> whether mx_linear quantises the activations on the way
 
     def __repr__(self):
         return f"MxTensor(shape={tuple(self.shape)}, device={self.device})"
@@ -1141,18 +1129,20 @@ def mx_quantize(x) -> MxTensor:
     2^(floor(log2 max) - 2) and the elements rounded half to even to 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (larger ones:
     6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros."""
     rows, ld = _token_rows(x, "x")
-    code, K = dtype_code(x.dtype), x.shape[-1]
+    code, K, dev = dtype_code(x.dtype), x.shape[-1], x.get_device()
     if K < 1:
         raise ValueError("mx_quantize: no elements to scale (K = 0)")
-    lib = _lib.load()
-    with _OnDevice(x.get_device()):
-        nc = lib.unetk_mx_codes_bytes(rows, K) if rows else 0
-        if rows and not nc:
-            raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
-        codes = torch.empty(nc, dtype=torch.uint8, device=x.device)
-        scales = torch.empty(nc // 16, dtype=torch.uint8, device=x.device)
-        if rows:
-            call("unetk_mx_quantize", _at(x), ld, rows, K, code, _at(codes), _at(scales), stream())
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return mx_quantize(x)
+    nc = _lib.load().unetk_mx_codes_bytes(rows, K) if rows else 0
+    if rows and not nc:
+        raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
+    both = torch.empty(nc + nc // 16, dtype=torch.uint8, device=x.device)
+    codes, scales = both[:nc], both[nc:]
+    if rows:
+        at = both.data_ptr()
+        call("unetk_mx_quantize", x.data_ptr(), ld, rows, K, code, at, at + nc, stream())
     return MxTensor(codes, scales, x.shape)
 
 
@@ -1160,11 +1150,13 @@ def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, exact in float32 and in bfloat16."""
     if not isinstance(q, MxTensor):
         raise TypeError(f"mx_dequantize: expected an MxTensor, got {type(q).__name__}")
-    code, rows, K = dtype_code(dtype), q.rows, q.shape[-1]
-    with _OnDevice(q.device.index):
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
-        if rows:
-            call("unetk_mx_dequantize", _at(q.codes), _at(q.scales), rows, K, _at(out), K, code, stream())
+    code, K = dtype_code(dtype), q.shape[-1]
+    if q.index != _raw_device():
+        with torch.cuda.device(q.index):
+            return mx_dequantize(q, dtype)
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if q.rows:
+        call("unetk_mx_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, K, out.data_ptr(), K, code, stream())
     return out
 
 
@@ -1173,46 +1165,56 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
     gradient).  x (..., K): a float32 or bfloat16 tensor, quantised on the way, or an MxTensor (quantised once for
     several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none, 2 GELU (erf form);
     resid: (..., N) of the result's type.  The result has x's type (``dtype`` for an MxTensor, bfloat16 if not given); out:
-    a (..., N) tensor or channel slice to write it to."""
+    a (..., N) tensor or channel slice to write it to (it may be resid itself, but share no memory with x)."""
     if not isinstance(w, MxTensor) or len(w.shape) != 2:
         raise TypeError("mx_linear: w is mx_quantize of the (N, K) weight")
     N, K = w.shape
+    dev = w.index
     quantised = isinstance(x, MxTensor)
-    if not quantised and not isinstance(x, torch.Tensor):
-        raise TypeError(f"mx_linear: x is a tensor or an MxTensor, not {type(x).__name__}")
-    if len(x.shape) < 1 or x.shape[-1] != K:
-        raise ValueError(f"mx_linear: x {tuple(x.shape)} against w {tuple(w.shape)}")
-    if x.device != w.device:
-        raise ValueError(f"mx_linear: x on {x.device}, w on {w.device}")
-    if act not in (0, 2):
-        raise ValueError(f"mx_linear: act {act!r} (0 none, 2 GELU)")
     if quantised:
         dt, rows = dtype or torch.bfloat16, x.rows
+        if x.index != dev:
+            raise ValueError(f"mx_linear: x on {x.device}, w on {w.device}")
     else:
-        if dtype is not None and dtype != x.dtype:
-            raise ValueError(f"mx_linear: dtype {dtype} for x of {x.dtype}")
+        rows, ldx = _token_rows(x, "x", dev)
         dt = x.dtype
-        rows, ldx = _token_rows(x, "x")
-    code, shape, dev = dtype_code(dt), x.shape[:-1] + (N,), w.device
-    bias = _vector(bias, "bias", N, dev.index)
+        if dtype is not None and dtype != dt:
+            raise ValueError(f"mx_linear: dtype {dtype} for x of {dt}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != K:
+        raise ValueError(f"mx_linear: x {tuple(shape)} against w {tuple(w.shape)}")
+    if act != 0 and act != 2:
+        raise ValueError(f"mx_linear: act {act!r} (0 none, 2 GELU)")
+    code = dtype_code(dt)
+    bias_at = _vector(bias, "bias", N, dev)
     ldo = ldr = N
-    for t, what in ((out, "out"), (resid, "resid")):
-        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != shape):
-            raise ValueError(f"{what}: expected the shape {tuple(shape)}")
-    if out is not None:
-        ldo = _token_rows(out, "out", dev.index, dt)[1]
-    if resid is not None:
-        ldr = _token_rows(resid, "resid", dev.index, dt)[1]
-    with _OnDevice(dev.index):
-        if out is None:
-            out = torch.empty(shape, dtype=dt, device=dev)
-        if rows and N:
-            lib = _lib.load()
-            if not quantised and lib.unetk_mx_linear_x_supported(rows, K, N, code):
-                call("unetk_mx_linear_x", x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, rows,
-                     K, N, bias, act, _at(resid), ldr, code, stream())
-            else:
-                xq = x if quantised else mx_quantize(x)
-                call("unetk_mx_linear", xq.codes.data_ptr(), xq.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-                     out.data_ptr(), ldo, rows, K, N, bias, act, _at(resid), ldr, code, stream())
+    if out is not None or resid is not None:
+        want = shape[:-1] + (N,)
+        for t, what in ((out, "out"), (resid, "resid")):
+            if t is not None and (not isinstance(t, torch.Tensor) or t.shape != want):
+                raise ValueError(f"{what}: expected the shape {tuple(want)}")
+        if out is not None:
+            ldo = _token_rows(out, "out", dev, dt)[1]
+        if resid is not None:
+            ldr = _token_rows(resid, "resid", dev, dt)[1]
+    if dev != _raw_device():
+        with torch.cuda.device(dev):
+            return mx_linear(x, w, bias, act, resid, out, dtype)
+    if out is None:
+        out = torch.empty(shape[:-1] + (N,), dtype=dt, device=w.device)
+    if rows and N:
+        fused = False
+        if not quantised:
+            fused = w._fused.get((rows, code))
+            if fused is None:
+                if len(w._fused) > 256:
+                    w._fused.clear()
+                fused = w._fused[(rows, code)] = bool(_lib.load().unetk_mx_linear_x_supported(rows, K, N, code))
+        if fused:
+            call("unetk_mx_linear_x", x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, rows,
+                 K, N, bias_at, act, _at(resid), ldr, code, stream())
+        else:
+            xq = x if quantised else mx_quantize(x)
+            call("unetk_mx_linear", xq.codes.data_ptr(), xq.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
+                 out.data_ptr(), ldo, rows, K, N, bias_at, act, _at(resid), ldr, code, stream())
     return out

@@ -8,6 +8,10 @@ kernel run as a 1x1 convolution (bias / residual / DropPath scale in its epilogu
 is one fused kernel per direction, and the CNN decoder reuses the conv + BatchNorm + ReLU kernels of
 the UNet.  Window size 8 and head dimension 32 (every stage of the reference configuration) are what
 the attention kernel implements; other values raise ValueError.
+
+Two configuration keys go beyond the reference: ``post_norm`` (a LayerNorm behind each branch of a block) and
+``layer_scale`` (a learned factor per channel on each branch, from this value on); without them the parameters and
+results are the reference's.  ``quantize_linears()`` predicts with the token linears in microscaled 4 bits.
 """
 import math
 import os
@@ -60,7 +64,9 @@ class WindowAttention(nn.Module):
 
 class SwinTransformerBlock(nn.Module):
     def __init__(self, dim, num_heads, window_size=7, shift_size=0, mlp_ratio=4., qkv_bias=True, drop=0.,
-                 attn_drop=0., drop_path=0.):
+                 attn_drop=0., drop_path=0., post_norm=False, layer_scale=None):
+        """post_norm: a LayerNorm behind each branch; layer_scale: a factor per channel on each branch, from this
+        value on (None: no factors).  Neither is in the reference: without them the block is its."""
         super().__init__()
         self.dim, self.num_heads, self.window_size, self.shift_size = dim, num_heads, window_size, shift_size
         self.mlp_ratio = mlp_ratio
@@ -72,6 +78,11 @@ class SwinTransformerBlock(nn.Module):
         hid = int(dim * mlp_ratio)
         self.mlp = nn.Sequential(nn.Linear(dim, hid), nn.GELU(), nn.Dropout(drop), nn.Linear(hid, dim),
                                  nn.Dropout(drop))
+        self.gated = bool(post_norm) or layer_scale is not None
+        self.post_norm1 = nn.LayerNorm(dim) if post_norm else None
+        self.post_norm2 = nn.LayerNorm(dim) if post_norm else None
+        self.gate1 = nn.Parameter(torch.full((dim,), float(layer_scale))) if layer_scale is not None else None
+        self.gate2 = nn.Parameter(torch.full((dim,), float(layer_scale))) if layer_scale is not None else None
 
 
 class PatchMerging(nn.Module):
@@ -84,14 +95,14 @@ class PatchMerging(nn.Module):
 
 class BasicLayer(nn.Module):
     def __init__(self, dim, depth, num_heads, window_size, mlp_ratio=4., qkv_bias=True, drop=0., attn_drop=0.,
-                 drop_path=0., downsample=None):
+                 drop_path=0., downsample=None, post_norm=False, layer_scale=None):
         super().__init__()
         self.dim, self.depth, self.window_size = dim, depth, window_size
         self.shift_size = window_size // 2
         self.blocks = nn.ModuleList([
             SwinTransformerBlock(dim, num_heads, window_size, 0 if i % 2 == 0 else self.shift_size, mlp_ratio,
                                  qkv_bias, drop, attn_drop,
-                                 drop_path[i] if isinstance(drop_path, list) else drop_path)
+                                 drop_path[i] if isinstance(drop_path, list) else drop_path, post_norm, layer_scale)
             for i in range(depth)])
         self.downsample = downsample(dim=dim) if downsample is not None else None
 
@@ -147,7 +158,7 @@ class SwinUNet(nn.Module):
             self.layers.append(BasicLayer(
                 dim, self.depths[i], self.num_heads[i], self.window_size, self.mlp_ratio, True, self.drop_rate,
                 self.attn_drop_rate, dpr[sum(self.depths[:i]):sum(self.depths[:i + 1])],
-                PatchMerging if i < self.num_layers - 1 else None))
+                PatchMerging if i < self.num_layers - 1 else None, c.get("post_norm", False), c.get("layer_scale")))
             if i < self.num_layers - 1:
                 dim = int(dim * 2)
         self.decoder_channels_conf = c["decoder_channels"]
@@ -164,6 +175,7 @@ class SwinUNet(nn.Module):
         self.drop_path_override: Optional[List] = None
         # data-parallel hook, see unet_amd.dist.GradReducer
         self.grad_sink = None
+        self._mx_linears = None         # quantize_linears()
 
     def _init_weights(self, m):
         # reference swin_unet_model.py:616-630 (ConvTranspose2d is not a Conv2d: keeps its default init)
@@ -178,6 +190,27 @@ class SwinUNet(nn.Module):
             nn.init.kaiming_normal_(m.weight, mode="fan_out", nonlinearity="relu")
             if m.bias is not None:
                 nn.init.constant_(m.bias, 0)
+
+    def quantize_linears(self):
+        """Prediction with the token linears (qkv, proj, fc1, fc2, patch merging) in microscaled 4 bits: their weights are
+        quantised now and kept beside the parameters, their inputs on the way (ops.mx_linear).  Eval mode only: training
+        steps use the parameters themselves.  A forward pass in eval mode raises once a quantised parameter has been
+        changed or moved; call this again (or dequantize_linears()) after that.  Returns self."""
+        weights = []
+        for layer in self.layers:
+            for blk in layer.blocks:
+                weights += [blk.attn.qkv.weight, blk.attn.proj.weight, blk.mlp[0].weight, blk.mlp[3].weight]
+            if layer.downsample is not None:
+                weights.append(layer.downsample.reduction.weight)
+        if not all(w.is_cuda for w in weights):
+            raise RuntimeError("quantize_linears: move the model to the GPU first")
+        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), w._version) for w in weights]
+        return self
+
+    def dequantize_linears(self):
+        """Back to the parameters themselves in eval mode.  Returns self."""
+        self._mx_linears = None
+        return self
 
     def late_grad_names(self):
         """Parameters whose gradients the backward pass completes with its closing launches (the LayerNorm weight /
@@ -246,7 +279,7 @@ class _Ctx:
     for training the data-gradient form) and looked up by the parameter's address; anything not
     found there (a reshaped copy) is packed on the spot.  Owned by the autograd node of the step
     (or dropped after an inference call): interleaved models or steps cannot see each other's packs."""
-    __slots__ = ("dt", "pool", "side", "fork", "held", "tracked", "sums")
+    __slots__ = ("dt", "pool", "side", "fork", "held", "tracked", "sums", "mx")
 
     def __init__(self, model, training):
         self.dt = dt = model.compute_dtype
@@ -255,6 +288,15 @@ class _Ctx:
         self.held = []
         self.tracked = []       # BatchNorm step counters of this forward: advanced by one launch at its end
         self.sums = None        # set by the backward pass: the LayerNorm parameter-gradient sums taken at its end
+        self.mx = None          # prediction with 4-bit linears: parameter address -> quantised weight
+        held = getattr(model, "_mx_linears", None)
+        if held is not None and not training:
+            self.mx = {}
+            for w, q, at, version in held:
+                if w.data_ptr() != at or w._version != version:
+                    raise RuntimeError("a SwinUNet parameter was changed or moved after quantize_linears(): call it again, "
+                                       "or dequantize_linears()")
+                self.mx[at] = q
         # (the walk over the module tree costs the host ~1 ms: its result is kept on the model, which does not
         # grow layers between steps; what can change - device, dtype, layout of a weight - is checked every time)
         cand = model.__dict__.get("_packable_modules")
@@ -425,6 +467,11 @@ def _linear_launch(x, pw, shift=None, act=0, resid=None, resid_keep=None, out=No
 
 # ------------------------------------------------------------------ building blocks
 def _linear(x, w, b, cx, act=0, resid=None, keep=None, out=None, out2=False):
+    if cx.mx is not None and keep is None:
+        q = cx.mx.get(w.data_ptr())
+        if q is not None and q.shape == w.shape:
+            y = ops.mx_linear(x, q, bias=b, act=act, resid=resid, out=out)
+            return (None, y) if out2 else y
     return _linear_launch(x, cx.packed(w), shift=b, act=act, resid=resid, resid_keep=keep, out=out, out2=out2)
 
 
@@ -478,7 +525,7 @@ def _block_fwd(blk, pre, x, keep1, keep2, cx, save):
     else:
         pr = _linear(att, a.proj.weight, a.proj.bias, cx)
         x1 = ops.scale_sample(pr[:, :H, :W].contiguous(), keep1, x)
-    p64 = cx.packed64(blk.mlp[0].weight) if FUSED_MLP else None
+    p64 = cx.packed64(blk.mlp[0].weight) if FUSED_MLP and cx.mx is None else None
     p96 = cx.packed(blk.mlp[3].weight) if p64 is not None else None
     if p64 is not None and p96.bn == 96 and blk.mlp[0].bias is not None and blk.mlp[3].bias is not None and \
             ops.swin_mlp_supported(x1):
@@ -487,7 +534,7 @@ def _block_fwd(blk, pre, x, keep1, keep2, cx, save):
                                                         want_act=FUSED_MLP_SAVE_ACT or save is None)
     else:
         ln2, m2, r2 = ops.layernorm_fwd(x1, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
-        if FUSE_GELU_FWD and hidden_small(x1, blk):
+        if cx.mx is not None or (FUSE_GELU_FWD and hidden_small(x1, blk)):
             # the deep stages (few tokens, wide layers): GELU as a second output of fc1's epilogue saves a launch
             # in a part of the step where launches, not bytes, set the time
             hpre, hact = _linear(ln2, blk.mlp[0].weight, blk.mlp[0].bias, cx, act=2, out2=True)
@@ -557,6 +604,88 @@ def _block_bwd(blk, pre, ctx, dx2, cx, grads, db2=None, keep_next=None):
                             scale_next=(keep_next, H * W) if (fuse and keep_next is not None) else None)
     dx, grads[pre + "norm1.weight"], grads[pre + "norm1.bias"] = res[:3]
     return dx, (res[3] if len(res) == 4 else None)
+
+
+def _norm_of(norm):
+    return None if norm is None else (norm.weight, norm.bias)
+
+
+def _gated_args(blk, which, nxt):
+    """Arguments of ops.gated_norm_fwd / _bwd at the end of a block's branch: its gate and the norm behind it, and the norm
+    in front of what follows."""
+    gate, post = (blk.gate1, blk.post_norm1) if which == 1 else (blk.gate2, blk.post_norm2)
+    return dict(gate=gate, post=_norm_of(post), pre=_norm_of(nxt), eps=blk.norm1.eps)
+
+
+def _gated_block_fwd(blk, pre, x, ln1, keep1, keep2, cx, save, nxt):
+    """A block with norms behind its branches or gates on them: x1 = x + keep1 * gate1 * post_norm1(attention), x2 = x1 +
+    keep2 * gate2 * post_norm2(MLP).  ln1: norm1(x), when the block in front left it (else formed here); nxt: name and
+    module of the next block's norm1, or None.  Returns (x2, nxt(x2) or None)."""
+    B, H, W, C = x.shape
+    ws = blk.window_size
+    _check_grid(H, W, ws)
+    He, We = max(H, ws), max(W, ws)
+    padded = (He, We) != (H, W)
+    a = blk.attn
+    own = None
+    if ln1 is None:
+        ln1, m1, r1 = ops.layernorm_fwd(x, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps)
+        own = (m1, r1)
+    ln1p = _pad_tokens(ln1, He, We)
+    qkv = _linear(ln1p, a.qkv.weight, a.qkv.bias, cx)
+    att = ops.window_attn_fwd(qkv, a.relative_position_bias_table, a.num_heads, blk.shift_size, True, ws=ws)
+    f1 = _linear(att, a.proj.weight, a.proj.bias, cx)
+    if padded:
+        f1 = f1[:, :H, :W].contiguous()
+    train = save is not None
+    x1, ln2, st1 = ops.gated_norm_fwd(x, f1, keep=keep1, want_stats=train, **_gated_args(blk, 1, blk.norm2))
+    if cx.mx is not None or (FUSE_GELU_FWD and hidden_small(x1, blk)):
+        hpre, hact = _linear(ln2, blk.mlp[0].weight, blk.mlp[0].bias, cx, act=2, out2=True)
+    else:
+        hpre = _linear(ln2, blk.mlp[0].weight, blk.mlp[0].bias, cx)
+        hact = ops.gelu_fwd(hpre)
+    f2 = _linear(hact, blk.mlp[3].weight, blk.mlp[3].bias, cx)
+    x2, ln_next, st2 = ops.gated_norm_fwd(x1, f2, keep=keep2, want_stats=train,
+                                          **_gated_args(blk, 2, nxt[1] if nxt is not None else None))
+    if train:
+        save.append(("gblock", blk, pre, nxt, (x, own, ln1p, qkv, att, f1, st1, x1, ln2, hpre, hact, f2, st2, keep1, keep2,
+                                               (H, W, He, We))))
+    return x2, ln_next
+
+
+def _gated_block_bwd(blk, pre, nxt, ctx, dx2, dnext, cx, grads):
+    """dx2: gradient of the block's output; dnext: gradient of nxt(x2), when the forward pass left that.  Returns (dx, dln1):
+    dln1 is the gradient of norm1(x) for the block in front, or None where this block formed norm1(x) itself (dx is then
+    complete)."""
+    x, own, ln1p, qkv, att, f1, st1, x1, ln2, hpre, hact, f2, st2, keep1, keep2, (H, W, He, We) = ctx
+    a = blk.attn
+    padded = (He, We) != (H, W)
+
+    def put(d, which, nname):
+        if d.gate is not None:
+            grads[f"{pre}gate{which}"] = d.gate
+        if d.post_weight is not None:
+            grads[f"{pre}post_norm{which}.weight"], grads[f"{pre}post_norm{which}.bias"] = d.post_weight, d.post_bias
+        if d.pre_weight is not None:
+            grads[nname + ".weight"], grads[nname + ".bias"] = d.pre_weight, d.pre_bias
+    d = ops.gated_norm_bwd(dx2, dnext, x1, f2, st2, keep=keep2, **_gated_args(blk, 2, nxt[1] if nxt is not None else None))
+    put(d, 2, nxt[0] if nxt is not None else None)
+    dhp = _linear_bwd(hact, d.f, blk.mlp[3].weight, cx, grads, pre + "mlp.3.weight", pre + "mlp.3.bias", gelu_grad_of=hpre)
+    dln2 = _linear_bwd(ln2, dhp, blk.mlp[0].weight, cx, grads, pre + "mlp.0.weight", pre + "mlp.0.bias")
+    d = ops.gated_norm_bwd(d.x, dln2, x, f1, st1, keep=keep1, **_gated_args(blk, 1, blk.norm2))
+    put(d, 1, pre + "norm2")
+    df1 = _pad_tokens(d.f, He, We) if padded else d.f
+    datt = _linear_bwd(att, df1, a.proj.weight, cx, grads, pre + "attn.proj.weight", pre + "attn.proj.bias")
+    dqkv, grads[pre + "attn.relative_position_bias_table"] = ops.window_attn_bwd(
+        qkv, datt, a.relative_position_bias_table, a.num_heads, blk.shift_size, True, defer=cx.sums, ws=blk.window_size)
+    dln1 = _linear_bwd(ln1p, dqkv, a.qkv.weight, cx, grads, pre + "attn.qkv.weight", pre + "attn.qkv.bias")
+    if padded:
+        dln1 = dln1[:, :H, :W].contiguous()
+    if own is None:
+        return d.x, dln1
+    dx, grads[pre + "norm1.weight"], grads[pre + "norm1.bias"] = ops.layernorm_bwd(
+        dln1, x, blk.norm1.weight, own[0], own[1], add=d.x, defer=cx.sums)
+    return dx, None
 
 
 def _conv_bn_relu_fwd(conv, bn, t, cx, training, save, tag):
@@ -681,9 +810,14 @@ def _forward(model, x, drop_path, save):
     skips = []
     bno = 0
     for li, layer in enumerate(model.layers):
+        ln1 = None      # norm1 of the next block, when the block in front leaves it (gated blocks)
         for bi, blk in enumerate(layer.blocks):
             k1, k2 = drop_path[bno] if (training and drop_path is not None) else (None, None)
-            t = _block_fwd(blk, f"layers.{li}.blocks.{bi}.", t, k1, k2, cx, save)
+            if blk.gated:
+                nxt = (f"layers.{li}.blocks.{bi + 1}.norm1", layer.blocks[bi + 1].norm1) if bi + 1 < len(layer.blocks) else None
+                t, ln1 = _gated_block_fwd(blk, f"layers.{li}.blocks.{bi}.", t, ln1, k1, k2, cx, save, nxt)
+            else:
+                t = _block_fwd(blk, f"layers.{li}.blocks.{bi}.", t, k1, k2, cx, save)
             bno += 1
         skips.append(t)
         if layer.downsample is not None:
@@ -742,6 +876,7 @@ class _SwinTrainFn(torch.autograd.Function):
         g = None
         pending_skip = None
         g_scaled = None                  # g times the next block's DropPath factors, when its producer wrote it
+        dln1 = None                      # gated blocks: gradient of the norm1 that the block in front formed
         presummed = None                 # BatchNorm-backward sums of the next unit, when g's producer left them
         for ri in range(len(save) - 1, -1, -1):
             rec = save[ri]
@@ -784,6 +919,9 @@ class _SwinTrainFn(torch.autograd.Function):
                 keep_next = nxt[3][13] if (nxt is not None and nxt[0] == "block" and nxt[3][14] == c[14]) else None
                 g, g_scaled = _block_bwd(blk, pre, c, g, cx, grads, db2=g_scaled, keep_next=keep_next)
                 continue
+            elif kind == "gblock":
+                _, blk, pre, nxt, c = rec
+                g, dln1 = _gated_block_bwd(blk, pre, nxt, c, g, dln1, cx, grads)
             elif kind == "embed":
                 tok_in, t0, m0, r0 = rec[1]
                 E = model.embed_dim_val
