@@ -449,13 +449,14 @@ int unetk_mx_linear(const void* xcodes, const void* xscales, const void* wcodes,
                     int64_t M, int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
                     unetk_stream_t stream);
 
-/* The same from unquantised activations (M rows of K elements of `dtype`, ldx apart) in one launch,
- * for the problems that unetk_mx_linear_x_supported names: few rows, or short K under many rows.  Same bits as
- * unetk_mx_quantize followed by unetk_mx_linear. */
-int unetk_mx_linear_x_supported(int64_t M, int64_t K, int64_t N, int dtype);
+/* The same from unquantised activations (M rows of K elements of `dtype`, ldx apart): quantised inside the product where
+ * that is one launch (few rows, or short K under many rows), else first, into the workspace
+ * (unetk_mx_linear_x_workspace_bytes, 16-byte aligned; 0: none is taken).  Same bits as unetk_mx_quantize followed by
+ * unetk_mx_linear. */
+int64_t unetk_mx_linear_x_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype);
 int unetk_mx_linear_x(const void* x, int64_t ldx, const void* wcodes, const void* wscales, void* out, int64_t ldo, int64_t M,
                       int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
-                      unetk_stream_t stream);
+                      void* workspace, unetk_stream_t stream);
 
 /* ---- optimizer tail: clip_grad_norm_ + AdamW over a list of fp32 tensors ----------------
  * enhanced_training_multi_loss.py:758-763 (AdamW), :827-829 (clip_grad_norm_(1.0), step);

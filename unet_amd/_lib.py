@@ -129,8 +129,8 @@ _SIGNATURES = {
     "unetk_mx_scales_bytes": (L, [L, L]),
     "unetk_mx_quantize": (I, [P, L, L, L, I, P, P, P]),
     "unetk_mx_dequantize": (I, [P, P, L, L, P, L, I, P]),
-    "unetk_mx_linear_x_supported": (I, [L, L, L, I]),
-    "unetk_mx_linear_x": (I, [P, L, P, P, P, L, L, L, L, P, I, P, L, I, P]),
+    "unetk_mx_linear_x_workspace_bytes": (L, [L, L, L, I]),
+    "unetk_mx_linear_x": (I, [P, L, P, P, P, L, L, L, L, P, I, P, L, I, P, P]),
     "unetk_mx_linear": (I, [P, P, P, P, P, L, L, L, L, P, I, P, L, I, P]),
     "unetk_window_attn_any_supported": (I, [I, I]),
     "unetk_window_attn_any_fwd": (I, [P, P, P, I, I, I, I, I, I, I, I, F, I, P]),

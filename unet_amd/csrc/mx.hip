@@ -260,6 +260,40 @@ __device__ __forceinline__ void store_tile(const MxArgs& a, uint32_t m, uint32_t
   store8<T, ACT, WHOLE, 1>(a, m, n + 16, acc);
 }
 
+// A wave's 64 x 64 tile in bfloat16 through LDS (TILE_LDS bytes of its own): stores of eight rows x 128 bytes instead of 32
+// rows x 32 bytes (8192^3: 295 us for the whole call, 313 without; in mx_rows_kernel the LDS it takes costs waves, and
+// 262144 x 96 -> 384 went from 66 to 87 us).  cWX: half W of the columns, half X of the rows.
+constexpr int TILE_LDS = 64 * 144;
+template <bool ACT, bool WHOLE>
+__device__ __forceinline__ void store_through_lds(const MxArgs& a, uint32_t m0, uint32_t n0, int lane, const f32x16& c00,
+                                                  const f32x16& c01, const f32x16& c10, const f32x16& c11, char* lds) {
+  auto put = [&](const f32x16& c, int wf, int xf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      Vec16<bf16> v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = from_f32<bf16>(mx_act<bf16, ACT>(c[j * 8 + e]));
+      store16(reinterpret_cast<bf16*>(lds + (xf * 32 + frag_row(lane & 31)) * 144 + (wf * 32 + j * 16 + ((lane >> 5) << 3)) * 2), v);
+    }
+  };
+  put(c00, 0, 0);
+  put(c01, 0, 1);
+  put(c10, 1, 0);
+  put(c11, 1, 1);
+  // (the wave's own LDS operations are carried out in order; the compiler must not turn them round)
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint32_t n = n0 + (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t r = i * 8 + (lane >> 3), m = m0 + r;
+    const Vec16<bf16> v = load16(reinterpret_cast<const bf16*>(lds + r * 144 + (lane & 7) * 16));
+    if (m < a.M) store_part<WHOLE>(reinterpret_cast<bf16*>(a.out) + (int64_t)m * a.ldo + n, v, (int)(a.N - n));
+  }
+  __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // f(GELU or not, rows of whole 16-byte pieces or not) as constants: the branch is taken once a tile, not once an element
 template <typename F> __device__ __forceinline__ void with_epilogue(const MxArgs& a, F&& f) {
   std::integral_constant<bool, false> no;
@@ -550,11 +584,11 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_ke
     // (opaque: the compiler would otherwise move the multiplications in front of each row's store)
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(t.acc[i]));
-    with_epilogue(a, [&](auto act, auto vec) __attribute__((always_inline)) {
+    with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        store_tile<T, decltype(act)::value, decltype(vec)::value>(a, mg * 64 + (i & 1) * 32 + frag_row(lane & 31),
-                                                                  g * 64 + (i >> 1) * 32, lane, t.acc[i]);
+        store_tile<T, decltype(act)::value, decltype(whole)::value>(a, mg * 64 + (i & 1) * 32 + frag_row(lane & 31),
+                                                                    g * 64 + (i >> 1) * 32, lane, t.acc[i]);
     });
   }
 }
@@ -576,6 +610,7 @@ __device__ __forceinline__ uint32_t lds_address(const char* p) {
 }
 
 constexpr int LG_STAGE = 2 * (16 * 1024 + 1024);      // codes of 256 rows and 256 columns, their scales
+static_assert(3 * TILE_LDS <= LG_STAGE, "three waves' output tiles in a stage");
 
 template <typename T>
 __global__ __launch_bounds__(256, 1) void mx_large_kernel(MxArgs a) {
@@ -707,13 +742,24 @@ __global__ __launch_bounds__(256, 1) void mx_large_kernel(MxArgs a) {
   wait_vm_then_barrier<0, true>();      // nothing of this workgroup writes LDS after its end
 #pragma unroll
   for (int i = 0; i < 16; ++i) asm volatile("" : "+a"(acc[i / 4][i % 4]));
-  with_epilogue(a, [&](auto act, auto vec) __attribute__((always_inline)) {
+  with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
+    constexpr bool ACT = decltype(act)::value, WH = decltype(whole)::value;
+    if constexpr (sizeof(T) == 2) {
+      if (a.resid == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          store_through_lds<ACT, WH>(a, mt * 256 + wm * 128 + (i & 1) * 64, nt * 256 + wn * 128 + (i >> 1) * 64, lane,
+                                     acc[(i >> 1) * 2][(i & 1) * 2], acc[(i >> 1) * 2][(i & 1) * 2 + 1],
+                                     acc[(i >> 1) * 2 + 1][(i & 1) * 2], acc[(i >> 1) * 2 + 1][(i & 1) * 2 + 1],
+                                     wave < 3 ? st0 + wave * TILE_LDS : st1);
+        return;
+      }
+    }
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        store_tile<T, decltype(act)::value, decltype(vec)::value>(a, mt * 256 + wm * 128 + x * 32 + frag_row(lane & 31),
-                                                                  nt * 256 + wn * 128 + w * 32, lane, acc[w][x]);
+        store_tile<T, ACT, WH>(a, mt * 256 + wm * 128 + x * 32 + frag_row(lane & 31), nt * 256 + wn * 128 + w * 32, lane, acc[w][x]);
   });
 }
 
@@ -752,7 +798,7 @@ template <typename T, typename SRC, typename TILE> void launch_split(const MxArg
 }
 template <typename T, typename SRC> void launch_split_f(const MxArgs& a, hipStream_t stream) {
   if (a.M <= 16) launch_split<T, SRC, Tile16>(a, stream);
-  else if constexpr (std::is_same<SRC, float>::value) return;      // (never asked for: unetk_mx_linear_x_supported)
+  else if constexpr (std::is_same<SRC, float>::value) return;      // (never asked for: such activations are quantised first)
   else if (a.M <= 32) launch_split<T, SRC, Tile32>(a, stream);
   else launch_split<T, SRC, Tile64>(a, stream);
 }
@@ -887,21 +933,26 @@ int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
   return UNETK_OK;
 }
 
-/* Whether mx_linear quantises activations on the way (unetk_mx_linear_x) for this problem: a few rows, where the launch
- * counts, and short K, where the rows are kept in registers. */
-int unetk_mx_linear_x_supported(int64_t M, int64_t K, int64_t N, int dtype) {
-  if (M < 1 || K < 1 || N < 1 || M > MX_MAX_ROWS || N > MX_MAX_ROWS || K > MX_MAX_K) return 0;
-  if (K % (dtype == UNETK_BF16 ? 8 : 4) != 0) return 0;
-  return M <= (dtype == UNETK_BF16 ? 64 : 16) || plan_of(M, K, N) == ROWS;
+int64_t unetk_mx_linear_x_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
+  const int64_t codes = unetk_mx_codes_bytes(M, K);
+  if (codes == 0 || N < 1 || N > MX_MAX_ROWS) return 0;
+  // quantised inside the product: a few rows, where the launch counts, and short K, where 64 rows are kept in LDS
+  const bool inside = K % (dtype == UNETK_BF16 ? 8 : 4) == 0 && (M <= (dtype == UNETK_BF16 ? 64 : 16) || plan_of(M, K, N) == ROWS);
+  return inside ? 0 : codes + codes / 16;
 }
 
 int unetk_mx_linear_x(const void* x, int64_t ldx, const void* wcodes, const void* wscales, void* out, int64_t ldo, int64_t M,
                       int64_t K, int64_t N, const float* bias, int act, const void* resid, int64_t ldr, int dtype,
-                      hipStream_t stream) {
+                      void* workspace, hipStream_t stream) {
   UNETK_CHECK_ARG(x && ldx >= K, "mx_linear_x: null activations or overlapping rows");
-  UNETK_CHECK_ARG(unetk_mx_linear_x_supported(M, K, N, dtype), "mx_linear_x: %lld x %lld x %lld is quantised first", (long long)M,
-                  (long long)K, (long long)N);
-  return mx_linear_impl(x, ldx, nullptr, nullptr, wcodes, wscales, out, ldo, M, K, N, bias, act, resid, ldr, dtype, stream);
+  const int64_t ws = unetk_mx_linear_x_workspace_bytes(M, K, N, dtype);
+  if (ws == 0)
+    return mx_linear_impl(x, ldx, nullptr, nullptr, wcodes, wscales, out, ldo, M, K, N, bias, act, resid, ldr, dtype, stream);
+  UNETK_CHECK_ARG(workspace != nullptr, "mx_linear_x: this problem takes a workspace");
+  const char* scales = (const char*)workspace + unetk_mx_codes_bytes(M, K);
+  const int rc = unetk_mx_quantize(x, ldx, M, K, dtype, workspace, (void*)scales, stream);
+  if (rc != UNETK_OK) return rc;
+  return mx_linear_impl(nullptr, 0, workspace, scales, wcodes, wscales, out, ldo, M, K, N, bias, act, resid, ldr, dtype, stream);
 }
 
 int unetk_mx_linear(const void* xcodes, const void* xscales, const void* wcodes, const void* wscales, void* out, int64_t ldo,

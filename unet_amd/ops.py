@@ -1110,15 +1110,16 @@ class MxTensor:
     """A (..., K) tensor in microscaled 4-bit floating point (OCP MXFP4): blocks of 32 along K, E2M1 elements and one
     power-of-two scale a block, in the order in which the matrix instruction reads them.  Made by mx_quantize; read by
     mx_linear (activations or weights alike) and mx_dequantize."""
-    __slots__ = ("codes", "scales", "shape", "rows", "device", "index", "_fused")
+    __slots__ = ("data", "split", "shape", "rows", "device", "index", "_work")
 
-    def __init__(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, torch.Size(shape)
-        self.device, self.index = codes.device, codes.get_device()
+    def __init__(self, data, split, shape):
+        """data: one uint8 buffer, the codes in its first ``split`` bytes, the scales behind them."""
+        self.data, self.split, self.shape = data, split, torch.Size(shape)
+        self.device, self.index = data.device, data.get_device()
         self.rows = 1
         for v in self.shape[:-1]:
             self.rows *= v
-        self._fused = {}        # as a weight: (rows, type) -> whether mx_linear quantises the activations on the way
+        self._work = {}        # as a weight: (rows, type) -> bytes that mx_linear needs to quantise the activations first
 
     def __repr__(self):
         return f"MxTensor(shape={tuple(self.shape)}, device={self.device})"
@@ -1138,12 +1139,11 @@ def mx_quantize(x) -> MxTensor:
     nc = _lib.load().unetk_mx_codes_bytes(rows, K) if rows else 0
     if rows and not nc:
         raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
-    both = torch.empty(nc + nc // 16, dtype=torch.uint8, device=x.device)
-    codes, scales = both[:nc], both[nc:]
+    data = torch.empty(nc + nc // 16, dtype=torch.uint8, device=x.device)
     if rows:
-        at = both.data_ptr()
+        at = data.data_ptr()
         call("unetk_mx_quantize", x.data_ptr(), ld, rows, K, code, at, at + nc, stream())
-    return MxTensor(codes, scales, x.shape)
+    return MxTensor(data, nc, x.shape)
 
 
 def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
@@ -1156,7 +1156,8 @@ def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
             return mx_dequantize(q, dtype)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if q.rows:
-        call("unetk_mx_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, K, out.data_ptr(), K, code, stream())
+        at = q.data.data_ptr()
+        call("unetk_mx_dequantize", at, at + q.split, q.rows, K, out.data_ptr(), K, code, stream())
     return out
 
 
@@ -1203,18 +1204,18 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
     if out is None:
         out = torch.empty(shape[:-1] + (N,), dtype=dt, device=w.device)
     if rows and N:
-        fused = False
-        if not quantised:
-            fused = w._fused.get((rows, code))
-            if fused is None:
-                if len(w._fused) > 256:
-                    w._fused.clear()
-                fused = w._fused[(rows, code)] = bool(_lib.load().unetk_mx_linear_x_supported(rows, K, N, code))
-        if fused:
-            call("unetk_mx_linear_x", x.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), ldo, rows,
-                 K, N, bias_at, act, _at(resid), ldr, code, stream())
+        at = w.data.data_ptr()
+        if quantised:
+            xat = x.data.data_ptr()
+            call("unetk_mx_linear", xat, xat + x.split, at, at + w.split, out.data_ptr(), ldo, rows, K, N, bias_at, act,
+                 _at(resid), ldr, code, stream())
         else:
-            xq = x if quantised else mx_quantize(x)
-            call("unetk_mx_linear", xq.codes.data_ptr(), xq.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-                 out.data_ptr(), ldo, rows, K, N, bias_at, act, _at(resid), ldr, code, stream())
+            need = w._work.get((rows, code))
+            if need is None:
+                if len(w._work) > 256:
+                    w._work.clear()
+                need = w._work[(rows, code)] = _lib.load().unetk_mx_linear_x_workspace_bytes(rows, K, N, code)
+            work = torch.empty(need, dtype=torch.uint8, device=w.device) if need else None
+            call("unetk_mx_linear_x", x.data_ptr(), ldx, at, at + w.split, out.data_ptr(), ldo, rows, K, N, bias_at, act,
+                 _at(resid), ldr, code, _at(work), stream())
     return out
