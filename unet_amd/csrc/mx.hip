@@ -519,6 +519,9 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_ke
   typedef typename std::conditional<RAW, SRC, bf16>::type S;
   __shared__ u32x4 xl[KS][4][64];
   __shared__ uint8_t sl[KS][64][4];
+  // The bias of this workgroup's columns.  (Loaded from memory at the head of a group it would be waited for behind the
+  // stores of the group before: loads and stores share one counter.)
+  extern __shared__ float bias[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups are dealt round-robin to the 8 XCDs: XCD x takes the x-th eighth of the list (rows, columns), columns
   // fastest, so that the workgroups that read the same rows do so through the same L2
@@ -539,6 +542,8 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_ke
 #pragma unroll
   for (int k = 0; k < KS; ++k) refill(g0 + wave, k);
   const int W = blockDim.x >> 6;
+  for (uint32_t i = threadIdx.x; i < (g1 - g0) * 64; i += blockDim.x)
+    bias[i] = (a.bias != nullptr && g0 * 64 + i < a.N) ? a.bias[g0 * 64 + i] : 0.f;
 #pragma unroll 1
   for (int f = wave; f < 4; f += W) {
     const uint32_t row = mg * 64 + (f & 1) * 32 + frag_row(lane & 31);
@@ -573,8 +578,13 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_ke
 #pragma unroll 1
   for (uint32_t g = g0 + wave; g < g1; g += W) {
     Tile64 t;
-    t.acc[0] = t.acc[1] = bias16(a, g * 64, lane);
-    t.acc[2] = t.acc[3] = bias16(a, g * 64 + 32, lane);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float* b = bias + (g - g0) * 64 + w * 32 + ((lane >> 5) << 3);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t.acc[2 * w][i] = b[((i >> 3) << 4) + (i & 7)];
+      t.acc[2 * w + 1] = t.acc[2 * w];
+    }
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const u32x4 xf[4] = {xl[k][0][lane], xl[k][1][lane], xl[k][2][lane], xl[k][3][lane]};
@@ -813,7 +823,8 @@ template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stre
   const double ks = a.kt, resident = 256.0 * (a.kt == 1 ? 16 : a.kt <= 3 ? 12 : 8);
   uint32_t W = 4, splits = 1;
   double best = 1e30;
-  for (uint32_t s = 1; s <= 16 && s <= a.ngroups; ++s)
+  const uint32_t s0 = (a.ngroups + 127) / 128;      // (at most 128 groups a workgroup: 32 KB of bias)
+  for (uint32_t s = s0; s < s0 + 16 && s <= a.ngroups; ++s)
     for (uint32_t w = 2; w <= 8; ++w) {
       const uint32_t per = (a.ngroups + s - 1) / s, used = (a.ngroups + per - 1) / per;
       const double path = blocks * (used * ks * 1600.0 + a.ngroups * (800.0 + ks * 140.0)) / 256.0;
@@ -825,13 +836,14 @@ template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stre
   a.per = (a.ngroups + splits - 1) / splits;
   splits = (a.ngroups + a.per - 1) / a.per;
   const dim3 grid((blocks * splits + 7) / 8 * 8), threads(64 * W);
+  const unsigned lds = a.per * 256;      // the bias
   switch (a.kt) {
-    case 1: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 1>), grid, threads, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 2>), grid, threads, 0, stream, a); break;
-    case 3: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 3>), grid, threads, 0, stream, a); break;
-    case 4: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 4>), grid, threads, 0, stream, a); break;
-    case 5: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 5>), grid, threads, 0, stream, a); break;
-    default: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 6>), grid, threads, 0, stream, a); break;
+    case 1: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 1>), grid, threads, lds, stream, a); break;
+    case 2: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 2>), grid, threads, lds, stream, a); break;
+    case 3: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 3>), grid, threads, lds, stream, a); break;
+    case 4: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 4>), grid, threads, lds, stream, a); break;
+    case 5: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 5>), grid, threads, lds, stream, a); break;
+    default: hipLaunchKernelGGL((mx_rows_kernel<T, SRC, 6>), grid, threads, lds, stream, a); break;
   }
 }
 
