@@ -157,12 +157,44 @@ def test_layer_shapes(rows, K, N):
     check_linear(rows, K, N, BF, act=2, resid=False)
 
 
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("rows,K,N", [(3400, 900, 3100), (1000, 100, 10300), (1000, 200, 10300), (900, 300, 10304), (1000, 400, 10300),
+                                      (1000, 520, 10300), (3329, 1031, 3585)])
+def test_large_products(rows, K, N, dt):
+    """256 x 256 tiles: one to nine steps of K (the pipeline is four deep), ragged last tiles."""
+    check_linear(rows, K, N, dt, act=2)
+    check_linear(rows, K, N, dt, act=0, resid=False)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("K", [8, 100, 128, 136, 256, 300, 384, 500, 640, 700, 768])
+def test_many_rows_of_every_step_count(K, dt):
+    check_linear(1025 + K, K, 200, dt, act=2)
+    check_linear(1024, K, 77, dt, act=0, resid=False)
+
+
+def test_more_columns_than_a_workgroup_takes():
+    check_linear(1030, 64, 9000, BF, resid=False)
+
+
+@pytest.mark.parametrize("rows,K,N", [(1100, 200, 130), (1500, 700, 7000), (3400, 900, 3100), (20, 300, 40)])
+def test_nan_stays_in_its_rows_and_columns(rows, K, N):
+    from unet_amd import ops
+    x, w = make((rows, K), 1, BF), make((N, K), 2)
+    x[rows - 1, K - 1], x[5, 0] = float("nan"), float("inf")
+    w[N - 1, 3] = float("-inf")
+    y = ops.mx_linear(x.cuda(), ops.mx_quantize(w.cuda()), act=2).float().cpu()
+    bad = torch.zeros(rows, N, dtype=torch.bool)
+    bad[rows - 1], bad[5], bad[:, N - 1] = True, True, True
+    assert torch.equal(torch.isnan(y), bad)
+
+
 def test_products_are_exact_where_fp32_is():
     """Small whole numbers: every sum is exact, so the result is, whatever the order."""
     from unet_amd import ops
     g = torch.Generator().manual_seed(0)
     grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
-    for rows, K, N in [(1, 256, 64), (9, 160, 70), (100, 512, 260), (700, 384, 400)]:
+    for rows, K, N in [(1, 256, 64), (9, 160, 70), (30, 512, 50), (100, 512, 260), (1700, 384, 400), (3400, 1152, 3100)]:
         x = grid[torch.randint(0, 8, (rows, K), generator=g)] * (torch.randint(0, 2, (rows, K), generator=g) * 2 - 1)
         w = grid[torch.randint(0, 8, (N, K), generator=g)] * (torch.randint(0, 2, (N, K), generator=g) * 2 - 1)
         x[:, ::32], w[:, ::32] = 4.0, 6.0      # every block's scale is 1

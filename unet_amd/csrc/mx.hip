@@ -93,27 +93,19 @@ __device__ __forceinline__ void load_block(const T* row, int k0, int K, bool the
     x.v[j] = __builtin_bit_cast(u32x4, load_part<WHOLE>(row + k0 + j * E, there ? K - (k0 + j * E) : 0));
 }
 
-// One wave: 64 rows x 128 k, each lane whole blocks.  Bound by the read of x.
+// One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t rows, int K,
-                                                          uint32_t kt, uint64_t units, u32x4* __restrict__ codes,
-                                                          uint32_t* __restrict__ scales) {
-  const uint64_t unit = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= units) return;
-  const int lane = threadIdx.x & 63;
-  const uint32_t g = (uint32_t)(unit / kt);
-  const int k0 = (int)(unit % kt) * 128 + (lane >> 5) * 32;
-  uint32_t sc = 0;
-#pragma unroll
-  for (int f = 0; f < 4; ++f) {
-    const uint32_t row = g * 64 + (f & 1) * 32 + frag_row(lane & 31);
-    RawBlock<T> r;
-    load_block<T, WHOLE>(x + (int64_t)(row < rows ? row : 0) * ldx, k0 + (f >> 1) * 64, K, row < rows, r);
-    u32x4 c;
-    sc |= mx_block(r, c) << (8 * f);
-    codes[(unit * 4 + f) * 64 + lane] = c;
-  }
-  scales[unit * 64 + lane] = sc;
+                                                          uint32_t kt, u32x4* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const uint64_t unit = blockIdx.x;
+  const int lane = threadIdx.x & 63, f = threadIdx.x >> 6;
+  const uint32_t row = (uint32_t)(unit / kt) * 64 + (f & 1) * 32 + frag_row(lane & 31);
+  const int k0 = (int)(unit % kt) * 128 + (f >> 1) * 64 + (lane >> 5) * 32;
+  RawBlock<T> r;
+  load_block<T, WHOLE>(x + (int64_t)(row < rows ? row : 0) * ldx, k0, K, row < rows, r);
+  u32x4 c;
+  scales[(unit * 64 + lane) * 4 + f] = (uint8_t)mx_block(r, c);
+  codes[(unit * 4 + f) * 64 + lane] = c;
 }
 
 // value of a code times 2^(scale byte - 127); the bf16 result is exact, the fp32 one too
@@ -871,7 +863,7 @@ int mx_linear_impl(const void* x, int64_t ldx, const void* xcodes, const void* x
   UNETK_CHECK_ARG(aligned16(wcodes) && aligned16(wscales), "mx_linear: misaligned packed operand");
   UNETK_CHECK_ARG(act == 0 || act == 2, "mx_linear: activation %d", act);
   // (grids: one block axis per 16 columns, one per 16...64 rows)
-  UNETK_CHECK_ARG(N <= (int64_t)1 << 24 && (M <= (int64_t)1 << 21 || plan_of(M, K, N) != SPLIT), "mx_linear: %lld x %lld outputs",
+  UNETK_CHECK_ARG(N <= (int64_t)1 << 24 && M <= (int64_t)1 << 28 && (M <= (int64_t)1 << 21 || plan_of(M, K, N) != SPLIT), "mx_linear: %lld x %lld outputs",
                   (long long)M, (long long)N);
   MxArgs a = {};
   a.x = x; a.ldx = ldx;
@@ -903,12 +895,11 @@ int unetk_mx_quantize(const void* x, int64_t ldx, int64_t rows, int64_t K, int d
   UNETK_CHECK_ARG(x && codes && scales && ldx >= K && aligned16(codes) && aligned16(scales),
                   "mx_quantize: null or misaligned operand, or overlapping rows");
   const uint32_t kt = (uint32_t)((K + 127) / 128);
-  const uint64_t units = (uint64_t)units_of(rows, (int)K);
-  const dim3 grid((unsigned)((units + 3) / 4));
+  const dim3 grid((unsigned)units_of(rows, (int)K));
   const bool whole = K % (dtype == UNETK_BF16 ? 8 : 4) == 0;
 #define MX_QUANT(T, V)                                                                                                \
   hipLaunchKernelGGL((mx_quantize_kernel<T, V>), grid, dim3(256), 0, stream, (const T*)x, ldx, (uint32_t)rows, (int)K, kt, \
-                     units, (u32x4*)codes, (uint32_t*)scales)
+                     (u32x4*)codes, (uint8_t*)scales)
   if (dtype == UNETK_BF16) {
     if (whole) MX_QUANT(bf16, true);
     else MX_QUANT(bf16, false);
