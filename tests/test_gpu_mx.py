@@ -289,3 +289,8 @@ def test_refusals():
             f()
     with pytest.raises(RuntimeError):
         ops.mx_quantize(x.cpu())
+    y = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.mx_linear(y, qw)
+    with torch.no_grad():
+        ops.mx_linear(y, qw)

@@ -122,6 +122,29 @@ def test_without_the_options_nothing_is_added():
     assert list(SwinUNet(cfg).state_dict()) == list(swin_oracle.swin_template(cfg))
 
 
+def test_gradient_sink_gets_every_gradient_once():
+    x, _, _ = W.synthetic_batch(2, 4, 64, 64, seed=42)
+    m, _, cfg = build(torch.bfloat16, **OPTIONS[0])
+    m.train()
+    m.drop_path_override = [[None, None]] * sum(cfg["depths"])
+    m(x.cuda()).square().mean().backward()
+    plain = {k: p.grad.clone() for k, p in m.named_parameters()}
+    for p in m.parameters():
+        p.grad = None
+    seen = {}
+
+    def sink(name, t):
+        assert name not in seen
+        seen[name] = t.clone()      # (on the stream that made it)
+        return t
+    m.grad_sink = sink
+    m(x.cuda()).square().mean().backward()
+    torch.cuda.synchronize()
+    assert set(seen) == set(plain)
+    for k in ("layers.0.blocks.1.norm1.weight", "layers.2.blocks.3.gate2", "layers.1.blocks.0.post_norm1.bias"):
+        assert torch.equal(seen[k], plain[k]), k
+
+
 def test_gated_step_in_a_graph_matches_the_eager_one():
     from oracle import loss_oracle
     from unet_amd import FusedAdamW, MultiLossFunction

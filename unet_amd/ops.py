@@ -1181,6 +1181,8 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
         dt = x.dtype
         if dtype is not None and dtype != dt:
             raise ValueError(f"mx_linear: dtype {dtype} for x of {dt}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("mx_linear has no gradient: call it under torch.no_grad(), or detach x")
     shape = x.shape
     if len(shape) < 1 or shape[-1] != K:
         raise ValueError(f"mx_linear: x {tuple(shape)} against w {tuple(w.shape)}")
