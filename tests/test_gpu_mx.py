@@ -136,7 +136,8 @@ def check_linear(rows, K, N, dt, bias=True, act=0, resid=True, x=None, scale=1.0
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("rows,K,N", [(1, 1, 1), (1, 32, 16), (1, 4096, 4096), (2, 129, 65), (15, 768, 40), (16, 128, 128), (17, 96, 384),
                                       (33, 200, 200), (64, 384, 96), (65, 1000, 333), (127, 31, 129), (128, 256, 256),
-                                      (200, 2072, 1511), (513, 640, 136), (1037, 72, 30), (300, 8192, 64)])
+                                      (200, 2072, 1511), (513, 640, 136), (1037, 72, 30), (300, 8192, 64), (600, 1000, 700), (500, 64, 1100),
+                                      (700, 1500, 1001), (20, 900, 24600), (30000, 900, 33), (64, 800, 25000), (4100, 5, 1)])
 def test_product(rows, K, N, dt):
     check_linear(rows, K, N, dt)
 
@@ -158,7 +159,7 @@ def test_layer_shapes(rows, K, N):
 
 
 @pytest.mark.parametrize("dt", [F32, BF])
-@pytest.mark.parametrize("rows,K,N", [(3400, 900, 3100), (1000, 100, 10300), (1000, 200, 10300), (900, 300, 10304), (1000, 400, 10300),
+@pytest.mark.parametrize("rows,K,N", [(3400, 900, 3100), (500, 100, 13000), (1000, 200, 10300), (900, 300, 10304), (1000, 400, 10300),
                                       (1000, 520, 10300), (3329, 1031, 3585)])
 def test_large_products(rows, K, N, dt):
     """256 x 256 tiles: one to nine steps of K (the pipeline is four deep), ragged last tiles."""
@@ -169,15 +170,18 @@ def test_large_products(rows, K, N, dt):
 @pytest.mark.parametrize("dt", [F32, BF])
 @pytest.mark.parametrize("K", [8, 100, 128, 136, 256, 300, 384, 500, 640, 700, 768])
 def test_many_rows_of_every_step_count(K, dt):
-    check_linear(1025 + K, K, 200, dt, act=2)
-    check_linear(1024, K, 77, dt, act=0, resid=False)
+    few = (K + 127) // 128 * 512
+    check_linear(few + 65, K, 200, dt, act=2)
+    check_linear(few, K, 77, dt, act=0, resid=False)
+    check_linear(few - 1, K, 77, dt, act=0, resid=False)
 
 
 def test_more_columns_than_a_workgroup_takes():
     check_linear(1030, 64, 9000, BF, resid=False)
 
 
-@pytest.mark.parametrize("rows,K,N", [(1100, 200, 130), (1500, 700, 7000), (3400, 900, 3100), (20, 300, 40)])
+@pytest.mark.parametrize("rows,K,N", [(1100, 200, 130), (1500, 700, 7000), (3400, 900, 3100), (20, 300, 40),
+                                      (3200, 700, 130), (600, 1000, 700)])
 def test_nan_stays_in_its_rows_and_columns(rows, K, N):
     from unet_amd import ops
     x, w = make((rows, K), 1, BF), make((N, K), 2)

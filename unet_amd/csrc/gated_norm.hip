@@ -12,6 +12,11 @@
 // operations an element.  All arithmetic is fp32; r, n, dx, df are rounded once, when they are stored.  n comes from the
 // unrounded r (which is in registers), and the backward pass forms r again from x and f for the same reason: it reads
 // as many bytes as with a stored r.
+//
+// Measured (MI355X; a large copy reaches 5.0 TB/s here), bf16 unless noted: forward 262144 x 96 43.8 us (4.6 TB/s),
+// 65536 x 192 28.3 us (3.6; its operands are left half in the last cache by the backward pass before), 8192 x 4096 RMS
+// 57.1 us (4.7); backward 65536 x 192 31.8 us (4.7 TB/s), 8192 x 4096 78.6 us (5.1), each and then 8...9 us for the column
+// sums; 5003 x 1001 fp32 19.5, 26.9 and 7.8 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.7 us: a launch.
 #include "unaligned.h"
 
 namespace {
@@ -27,7 +32,7 @@ struct NormArgs {
   float* stats_out;      // [M][4]: mean and rstd of f, mean and rstd of r
   void* o0;              // r / dx
   void* o1;              // n / df
-  float* partials;       // [workgroups][5][C]
+  float* partials;       // [workgroups][4][C]
   uint32_t M, rps;       // rows; rows per sample
   int C, rms;
   float res_scale, eps;

@@ -93,7 +93,9 @@ __device__ __forceinline__ void load_block(const T* row, int k0, int K, bool the
     x.v[j] = __builtin_bit_cast(u32x4, load_part<WHOLE>(row + k0 + j * E, there ? K - (k0 + j * E) : 0));
 }
 
-// One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x.
+// One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x: 65536 x 768 bf16 28.7 us (127 MB,
+// 4.4 TB/s), 8192 x 8192 47 us (170 MB, 3.6 TB/s).  (One workgroup of four waves a unit: with a wave a unit, four fragments in
+// turn, a small matrix has too few waves to hide its loads.)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t rows, int K,
                                                           uint32_t kt, u32x4* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -121,7 +123,7 @@ __device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
 }
 
 // One workgroup a unit; a lane makes 8 consecutive values, 16 lanes the 128 of a row: runs of 256 bytes (bf16) a row.  Bound
-// by the write of the values.
+// by the write of the values: 65536 x 768 to bf16 22.8 us (127 MB, 5.6 TB/s: much of the codes still lies in the last cache).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             uint32_t rows, int K, uint32_t kt, T* __restrict__ out, int64_t ldo) {
@@ -301,7 +303,8 @@ template <typename F> __device__ __forceinline__ void with_epilogue(const MxArgs
 
 // ---- few tiles: the W waves of a workgroup share the steps of K of one tile of SIDE x SIDE outputs and add their sums
 // through LDS in a fixed tree.  SRC: the activations' own type, quantised by each wave for its steps, or void: packed.
-// A step's fragments are fetched one step ahead.
+// A step's fragments are fetched one step ahead.  Bound by latency: 1 x 4096 -> 4096 5.2 us replayed from a graph (8.9 MB of
+// weights, 1.8 us at 5 TB/s), 1037 x 2072 -> 1511 fp32 9 us.
 
 // one 16 x 16 tile (16x16x128: lane l holds row l % 16, k block l / 16), its fragments gathered from the units by blocks
 struct Tile16 {
@@ -337,36 +340,32 @@ struct Tile64 {
 };
 
 template <typename T, typename SRC, typename TILE>
-__global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel(MxArgs a) {
+__global__ __launch_bounds__(1024) void mx_split_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
   typedef typename std::conditional<RAW, SRC, bf16>::type S;
   constexpr int SIDE = TILE::SIDE, NF = TILE::NF, NA = TILE::NA;
   extern __shared__ f32x4 xch[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
-  const uint32_t n0 = blockIdx.x * SIDE, m0 = blockIdx.y * SIDE, ng = n0 >> 6, xg = m0 >> 6;
+  const uint32_t across = (a.N + SIDE - 1) / SIDE, mt = blockIdx.x / across, nt = blockIdx.x - mt * across;
+  const uint32_t n0 = nt * SIDE, m0 = mt * SIDE, ng = n0 >> 6, xg = m0 >> 6;
   // where this lane's blocks of fragment f lie in a unit (16-byte slots), for the rows from r0 (in the unit) on
   auto slot = [&](uint32_t r0, int f) __attribute__((always_inline)) -> int {
     if constexpr (SIDE == 16) return Tile16::unit_slot(lane, r0 + (lane & 15));
-    else if constexpr (SIDE == 32) return (f * 2 + (r0 >> 5)) * 64 + lane;
-    else return f * 64 + lane;
+    else return (f * 2 + (r0 >> 5)) * 64 + lane;
   };
   // row and first k (in the step) of this lane's block of fragment f, for activations quantised here: in a unit's order,
   // so that both sources give the same tile
   auto raw_row = [&](int f) __attribute__((always_inline)) -> uint32_t {
     if constexpr (SIDE == 16) return m0 + (lane & 15);
-    else if constexpr (SIDE == 32) return m0 + frag_row(lane & 31);
-    else return m0 + (f & 1) * 32 + frag_row(lane & 31);
+    else return m0 + frag_row(lane & 31);
   };
   auto raw_k = [&](int f) __attribute__((always_inline)) -> int {
     if constexpr (SIDE == 16) return (lane >> 4) * 32;
-    else if constexpr (SIDE == 32) return f * 64 + (lane >> 5) * 32;
-    else return (f >> 1) * 64 + (lane >> 5) * 32;
+    else return f * 64 + (lane >> 5) * 32;
   };
   // the scale bytes of this lane's blocks out of a unit's word(s), byte f: fragment f
   auto scales = [&](const uint32_t* unit, uint32_t r0) __attribute__((always_inline)) -> uint32_t {
-    if constexpr (SIDE == 64) {
-      return unit[lane];
-    } else if constexpr (SIDE == 32) {
+    if constexpr (SIDE == 32) {
       const uint32_t v = unit[lane] >> (8 * (r0 >> 5));      // fragments r0 / 32 and 2 + r0 / 32
       return (v & 255u) | (v >> 8 & 0xff00u);
     } else {
@@ -382,13 +381,10 @@ __global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel
       t.acc[0][i] = (wave == 0 && a.bias != nullptr && n < a.N) ? a.bias[n] : 0.f;
     }
   } else {
+    t.acc[0] = bias16(a, n0, lane);
+    if (wave != 0)
 #pragma unroll
-    for (int i = 0; i < NA / 4; ++i) {
-      t.acc[i] = bias16(a, n0 + (i >> 1) * 32, lane);
-      if (wave != 0)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) t.acc[i][j] = 0.f;
-    }
+      for (int j = 0; j < 16; ++j) t.acc[0][j] = 0.f;
   }
   struct Step {
     u32x4 w[NF], x[NF];
@@ -430,16 +426,16 @@ __global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel
   }
   auto part = [&](int i) __attribute__((always_inline)) -> f32x4 {
     if constexpr (SIDE == 16) return t.acc[0];
-    else return f32x4{t.acc[i / 4][i % 4 * 4], t.acc[i / 4][i % 4 * 4 + 1], t.acc[i / 4][i % 4 * 4 + 2], t.acc[i / 4][i % 4 * 4 + 3]};
+    else return f32x4{t.acc[0][i * 4], t.acc[0][i * 4 + 1], t.acc[0][i * 4 + 2], t.acc[0][i * 4 + 3]};
   };
-  // down to four waves (two for the small tiles) by halves, then each of those sums and finishes its share of the tile
-  constexpr int FIN = SIDE == 64 ? 4 : SIDE == 32 ? 2 : 1;
+  // down to two waves (one for 16 x 16) by halves, then each of those sums and finishes its share of the tile
+  constexpr int FIN = SIDE == 32 ? 2 : 1;
   const int left = W < FIN ? W : FIN, each = NA / left;
   auto add = [&](int i, const f32x4& v) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (SIDE == 16) t.acc[0][j] += v[j];
-      else t.acc[i / 4][i % 4 * 4 + j] += v[j];
+      else t.acc[0][i * 4 + j] += v[j];
     }
   };
   for (int half = W >> 1; half >= FIN; half >>= 1) {
@@ -469,7 +465,7 @@ __global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if constexpr (SIDE == 16) t.acc[0][j] = v[j];
-            else t.acc[i / 4][i % 4 * 4 + j] = v[j];
+            else t.acc[0][i * 4 + j] = v[j];
           }
         }
     }
@@ -486,16 +482,15 @@ __global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel
         reinterpret_cast<T*>(a.out)[(int64_t)m * a.ldo + n + i] = from_f32<T>(y);
       }
   } else {
-    // parts i, i + 1 (i even): 8 columns from col8(i) on of this lane's row in half i / 4 % 2 of the rows
-    auto col8 = [&](int i) __attribute__((always_inline)) -> uint32_t { return (i >> 3) * 32 + (i & 2) * 8 + ((lane >> 5) << 3); };
+    // parts i, i + 1 (i even): 8 consecutive columns of this lane's row
     with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < NA; i += 2) {
         if (wave >= left || i / each != wave) continue;
         f32x16 r;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = t.acc[i / 4][(i & 2) * 4 + (j & 7)];
-        store8<T, decltype(act)::value, decltype(whole)::value, 0>(a, m0 + ((i >> 2) & 1) * 32 + frag_row(lane & 31), n0 + col8(i), r);
+        for (int j = 0; j < 16; ++j) r[j] = t.acc[0][i * 4 + (j & 7)];
+        store8<T, decltype(act)::value, decltype(whole)::value, 0>(a, m0 + frag_row(lane & 31), n0 + i * 8 + ((lane >> 5) << 3), r);
       }
     });
   }
@@ -505,6 +500,10 @@ __global__ __launch_bounds__(TILE::SIDE == 64 ? 512 : 1024) void mx_split_kernel
 // waves take every W-th group of 64 columns.  The weights' fragments come straight from the caches into
 // a ring of registers, a group ahead; the rows' are read from LDS a step at a time.  Bound by the write of the output (a
 // store instruction whose lanes lie in many rows holds the CU's address path for some 100 cycles) and the arithmetic on it.
+// 262144 x 96 -> 384 with GELU: 61 us (45 without) into an output that stays in the last cache, 73 and 17 more until the
+// next kernel starts (the 32 MB in the L2 caches are written back then) into one that does not; a floor of 50.  16384 x
+// 384 -> 1152: 15.8 us (50 MB, 3.2 TB/s).  Stores past the caches (nontemporal) cost three times as much: the 32 bytes that
+// an instruction has of a row are no longer joined to lines.
 template <typename T, typename SRC, int KS>
 __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
@@ -781,28 +780,44 @@ int check_mx(const char* who, int64_t rows, int64_t K, int dtype) {
 }
 
 // Which kernel takes an M x N x K product: by sizes alone, so that activations quantised beforehand give the same bits.
+// Times in us, bf16, replayed from a graph.
+//   rows against quantisation and split (short K): 1024 x 192 -> 768 5.8 and 5.8, 2048 rows 6.0 and 6.6; x 384 -> 1152: 1024 rows
+//   7.2 and 6.8, 2048 7.6 and 8.1; x 768 -> 2304: 2048 rows 14.5 and 13.3, 4096 19.0 and 21.7: from 512 rows a step of K on;
+//   large against split: 64 tiles (2048 x 2048) 28.2 and 24.3 with K = 4096, 14.5 and 9.6 with 1024; 96 tiles (2048 x 3000) 28.9
+//   and 41.3, 15.1 and 14.2.  A side of 64 fills a quarter of its tiles: 64 x 4096 -> 65536 45.2 and 28.9, 65536 x 2048 -> 64 27.7
+//   and 24.8; of 128: 128 x 2048 -> 65536 29.6 and 38.0, 65536 x 1024 -> 128 21.8 and 25.8.
 enum Plan { SPLIT, ROWS, LARGE };
 Plan plan_of(int64_t M, int64_t K, int64_t N) {
   const int64_t kt = (K + 127) / 128;
-  if (kt <= 6 && M >= 1024) return ROWS;
-  if (((M + 255) / 256) * ((N + 255) / 256) >= 160) return LARGE;
+  if (kt <= 6 && M >= 512 * kt) return ROWS;
+  if (M > 64 && N > 64 && ((M + 255) / 256) * ((N + 255) / 256) >= 96) return LARGE;
   return SPLIT;
+}
+// the split kernel's tile, 16 or 32 a side: 32 x 4096 -> 4096 4.4 and 4.9 us, 64 x 4096 -> 4096 5.6 and 5.2, 256 x 1024 -> 1024 3.7
+// both, 512 x 4096 -> 512 5.6 and 5.2.  (64 a side: 1024 x 1024 -> 1024 7.5 against 4.7 with 32, 2048 x 4096 -> 2048 22.6 against 24.3.)
+bool small_tiles(int64_t M, int64_t N) { return M * N < 1 << 18; }
+// Activations quantised inside the product, by every tile of columns again, or by a launch of their own: bf16 4 x 4096 -> 4096
+// 5.7 and 6.1 us, 8 x 4096 -> 4096 6.3 and 6.1, 16 x 2048 -> 2048 5.2 and 5.7, 16 x 4096 -> 4096 7.8 and 6.2; fp32 1 x 4096 -> 4096 6.3
+// both, 16 x 1024 -> 1024 5.0 and 5.4, 4 x 4096 -> 4096 7.1 and 6.3.
+bool quantised_inside(int64_t M, int64_t K, int64_t N, int dtype) {
+  if (K % (dtype == UNETK_BF16 ? 8 : 4) != 0) return false;
+  const Plan p = plan_of(M, K, N);
+  if (p != SPLIT) return p == ROWS;
+  return dtype == UNETK_BF16 ? M * K <= 32768 : M * K <= 16384 && small_tiles(M, N);
 }
 
 template <typename T, typename SRC, typename TILE> void launch_split(const MxArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)cdiv(a.N, TILE::SIDE), (unsigned)cdiv(a.M, TILE::SIDE));
-  // waves a tile: about 4096 in all, at least a step each
-  const int64_t tiles = (int64_t)grid.x * grid.y;
+  // waves a tile: about 2048 in all, at least a step each (256 x 4096 -> 4096: 9.5 us with 1024, 7.7 with 2048, 8.7 with 4096; 1 x
+  // 4096 -> 4096 4.1, 3.7, 4.0)
+  const int64_t tiles = ((a.M + TILE::SIDE - 1) / TILE::SIDE) * (int64_t)((a.N + TILE::SIDE - 1) / TILE::SIDE);
   int W = 1;
-  while (W < (TILE::SIDE == 64 ? 8 : 16) && tiles * W < 4096 && (uint32_t)W * 2 <= a.kt) W *= 2;
-  const int fin = TILE::SIDE == 64 ? 4 : TILE::SIDE == 32 ? 2 : 1, parts = W / 2 > fin ? W / 2 : W < fin ? W : fin;
-  hipLaunchKernelGGL((mx_split_kernel<T, SRC, TILE>), grid, dim3(64 * W), W > 1 ? parts * TILE::NA * 1024 : 0, stream, a);
+  while (W < 16 && tiles * W < 2048 && (uint32_t)W * 2 <= a.kt) W *= 2;
+  const int fin = TILE::SIDE == 32 ? 2 : 1, parts = W / 2 > fin ? W / 2 : W < fin ? W : fin;
+  hipLaunchKernelGGL((mx_split_kernel<T, SRC, TILE>), dim3((unsigned)tiles), dim3(64 * W), W > 1 ? parts * TILE::NA * 1024 : 0, stream, a);
 }
 template <typename T, typename SRC> void launch_split_f(const MxArgs& a, hipStream_t stream) {
-  if (a.M <= 16) launch_split<T, SRC, Tile16>(a, stream);
-  else if constexpr (std::is_same<SRC, float>::value) return;      // (never asked for: such activations are quantised first)
-  else if (a.M <= 32) launch_split<T, SRC, Tile32>(a, stream);
-  else launch_split<T, SRC, Tile64>(a, stream);
+  if (small_tiles(a.M, a.N)) launch_split<T, SRC, Tile16>(a, stream);
+  else if constexpr (!std::is_same<SRC, float>::value) launch_split<T, SRC, Tile32>(a, stream);      // (floats: never asked for)
 }
 
 template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stream) {
@@ -811,7 +826,8 @@ template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stre
   // How many waves share 64 rows, and over how many workgroups their columns are split, from what bounds the kernel, in
   // cycles of a CU: its address path (about 100 for a load or store whose lanes lie in many rows: 16 of a step's rows, 8 of a
   // group's results; 33 for 1 KB of weights), and the rounds of resident workgroups times a wave's own way through its
-  // share.  (16384 x 384 -> 1152: 20.2 us as picked here, 25.9 with three waves and six splits, which has the fewer rounds.)
+  // share.  (16384 x 384 -> 1152 is 15.8 us as picked; when it was 20.2, three waves and six splits, which has the fewer rounds,
+  // took 25.9.)
   const double ks = a.kt, resident = 256.0 * (a.kt == 1 ? 16 : a.kt <= 3 ? 12 : 8);
   uint32_t W = 4, splits = 1;
   double best = 1e30;
@@ -862,8 +878,8 @@ int mx_linear_impl(const void* x, int64_t ldx, const void* xcodes, const void* x
                   "mx_linear: null operand or overlapping rows");
   UNETK_CHECK_ARG(aligned16(wcodes) && aligned16(wscales), "mx_linear: misaligned packed operand");
   UNETK_CHECK_ARG(act == 0 || act == 2, "mx_linear: activation %d", act);
-  // (grids: one block axis per 16 columns, one per 16...64 rows)
-  UNETK_CHECK_ARG(N <= (int64_t)1 << 24 && M <= (int64_t)1 << 28 && (M <= (int64_t)1 << 21 || plan_of(M, K, N) != SPLIT), "mx_linear: %lld x %lld outputs",
+  // (a launch has fewer than 2^32 lanes)
+  UNETK_CHECK_ARG(N <= (int64_t)1 << 24 && M <= (int64_t)1 << 28 && M * N <= (int64_t)1 << 39, "mx_linear: %lld x %lld outputs",
                   (long long)M, (long long)N);
   MxArgs a = {};
   a.x = x; a.ldx = ldx;
@@ -939,9 +955,7 @@ int unetk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
 int64_t unetk_mx_linear_x_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
   const int64_t codes = unetk_mx_codes_bytes(M, K);
   if (codes == 0 || N < 1 || N > MX_MAX_ROWS) return 0;
-  // quantised inside the product: a few rows, where the launch counts, and short K, where 64 rows are kept in LDS
-  const bool inside = K % (dtype == UNETK_BF16 ? 8 : 4) == 0 && (M <= (dtype == UNETK_BF16 ? 64 : 16) || plan_of(M, K, N) == ROWS);
-  return inside ? 0 : codes + codes / 16;
+  return quantised_inside(M, K, N, dtype) ? 0 : codes + codes / 16;
 }
 
 int unetk_mx_linear_x(const void* x, int64_t ldx, const void* wcodes, const void* wscales, void* out, int64_t ldo, int64_t M,
