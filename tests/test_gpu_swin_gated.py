@@ -236,6 +236,48 @@ def test_changed_weights_are_refused_until_quantised_again():
     assert torch.equal(m(x.cuda()), t)
 
 
+def test_trained_weights_are_refused_until_quantised_again():
+    """The optimizer's kernel writes the parameters without autograd's knowledge, and a captured step without Python's."""
+    import unet_amd
+    from unet_amd.graph import GraphedTrainStep
+    x, y, _ = W.synthetic_batch(1, 4, 64, 64, seed=42)
+    x, y = x.cuda(), y.cuda()
+    m, _, _ = build(torch.bfloat16)
+
+    def predict():
+        m.eval()
+        with torch.no_grad():
+            return m(x)
+
+    def loss(out, label):
+        return ((out - F.interpolate(label, out.shape[-2:])) ** 2).mean()
+
+    m.quantize_linears()
+    a = predict()
+    opt = unet_amd.FusedAdamW(m.parameters(), lr=1e-2, capturable=True)
+    assert torch.equal(predict(), a)      # an optimizer alone changes nothing
+    m.train()
+    loss(m(x), y).backward()
+    opt.step()
+    with pytest.raises(RuntimeError, match="quantize_linears"):
+        predict()
+    m.quantize_linears()
+    assert not torch.equal(predict(), a)
+    m.train()
+    step = GraphedTrainStep(m, loss, opt, x, y, warmup=2)
+    m.quantize_linears()
+    b = predict()
+    m.train()
+    for _ in range(2):
+        step(x, y)
+        with pytest.raises(RuntimeError, match="quantize_linears"):
+            predict()
+        m.quantize_linears()
+        c = predict()
+        assert not torch.equal(b, c)
+        b = c
+
+
 def test_one_block_of_operators_together():
     """The chain that a prediction runs: norm -> 4-bit product -> 4-bit product with GELU -> norm with gate and residual,
     against 64 bits on the operators' own intermediate values."""

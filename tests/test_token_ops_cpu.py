@@ -96,3 +96,18 @@ def test_host_tensors_are_refused():
     for f in (lambda: ops.gated_norm_fwd(x, x, pre=(w, w)), lambda: ops.mx_quantize(x)):
         with pytest.raises(RuntimeError, match="GPU"):
             f()
+
+
+def test_steps_of_an_optimizer_are_known_to_its_parameters():
+    import unet_amd
+    from unet_amd.optim import steps_taken
+    a, b = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    one = unet_amd.FusedAdamW([a], lr=1e-3)
+    two = unet_amd.FusedAdamW([{"params": [a]}], lr=1e-3)
+    two.add_param_group({"params": [b]})
+    assert steps_taken(a) == steps_taken(b) == steps_taken(torch.zeros(1)) == 0
+    one.step()      # (no gradient is there: nothing is launched)
+    assert (steps_taken(a), steps_taken(b)) == (1, 0)
+    two.step()
+    two.step()
+    assert (steps_taken(a), steps_taken(b)) == (3, 2)

@@ -73,6 +73,7 @@ class GraphedTrainStep:
         if self.w is not None and w is not None and w.data_ptr() != self.w.data_ptr():
             self.w.copy_(w, non_blocking=True)
         self.optimizer.sync_hyper()
+        self.optimizer._steps[0] += 1
         self.graph.replay()
         parts = _LossParts(*self._parts_src) if self._parts_src is not None else self._parts
         return self.loss, parts

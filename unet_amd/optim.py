@@ -92,6 +92,12 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_ty
     return out[0]
 
 
+def steps_taken(p) -> int:
+    """How many steps FusedAdamW optimizers have taken over this parameter (its kernel writes past autograd's version
+    counter): for what is derived from a parameter and kept beside it."""
+    return sum(n[0] for n in getattr(p, "_unetk_steps", ()))
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW semantics (decoupled weight decay, bias correction), one launch per group.
 
@@ -106,6 +112,7 @@ class FusedAdamW(torch.optim.Optimizer):
         changed by a scheduler reaches the device through ``sync_hyper()``."""
         if lr < 0 or eps < 0 or not (0 <= betas[0] < 1) or not (0 <= betas[1] < 1) or weight_decay < 0:
             raise ValueError("invalid AdamW hyper-parameter")
+        self._steps = [0]       # steps taken, replays of a captured one among them: shared with the parameters
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None
@@ -113,6 +120,12 @@ class FusedAdamW(torch.optim.Optimizer):
         self._lists = {}
         self._fast = {}         # group index -> what step() keeps between calls (see there)
         self._hyper = {}        # group index -> (hyper double[5] on the device, dyn float[3], last pushed (lr, wd, betas))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if not any(n is self._steps for n in getattr(p, "_unetk_steps", ())):
+                p._unetk_steps = getattr(p, "_unetk_steps", []) + [self._steps]
 
     # ------------------------------------------------------------------ device-resident step / lr (capturable)
     def _hyper_for(self, gi, group, device):
@@ -228,6 +241,7 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        self._steps[0] += 1
         loss = None
         if closure is not None:
             with torch.enable_grad():

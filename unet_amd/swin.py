@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib, ops
+from .optim import steps_taken
 
 _WS = 8
 # GELU' inside the epilogue of fc2's data gradient: on the wide token grids it saves a write and a read of the hidden
@@ -195,7 +196,8 @@ class SwinUNet(nn.Module):
         """Prediction with the token linears (qkv, proj, fc1, fc2, patch merging) in microscaled 4 bits: their weights are
         quantised now and kept beside the parameters, their inputs on the way (ops.mx_linear).  Eval mode only: training
         steps use the parameters themselves.  A forward pass in eval mode raises once a quantised parameter has been
-        changed or moved; call this again (or dequantize_linears()) after that.  Returns self."""
+        changed or moved; call this again (or dequantize_linears()) after that.  (Seen are changes that count in autograd's
+        version counter, and FusedAdamW's steps, replayed ones too; not writes through ``parameter.data``.)  Returns self."""
         weights = []
         for layer in self.layers:
             for blk in layer.blocks:
@@ -204,7 +206,7 @@ class SwinUNet(nn.Module):
                 weights.append(layer.downsample.reduction.weight)
         if not all(w.is_cuda for w in weights):
             raise RuntimeError("quantize_linears: move the model to the GPU first")
-        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), w._version) for w in weights]
+        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), (w._version, steps_taken(w))) for w in weights]
         return self
 
     def dequantize_linears(self):
@@ -293,7 +295,7 @@ class _Ctx:
         if held is not None and not training:
             self.mx = {}
             for w, q, at, version in held:
-                if w.data_ptr() != at or w._version != version:
+                if w.data_ptr() != at or (w._version, steps_taken(w)) != version:
                     raise RuntimeError("a SwinUNet parameter was changed or moved after quantize_linears(): call it again, "
                                        "or dequantize_linears()")
                 self.mx[at] = q
