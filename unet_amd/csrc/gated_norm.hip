@@ -13,10 +13,10 @@
 // unrounded r (which is in registers), and the backward pass forms r again from x and f for the same reason: it reads
 // as many bytes as with a stored r.
 //
-// Measured (MI355X; a large copy reaches 5.0 TB/s here), bf16 unless noted: forward 262144 x 96 43.8 us (4.6 TB/s),
-// 65536 x 192 28.3 us (3.6; its operands are left half in the last cache by the backward pass before), 8192 x 4096 RMS
-// 57.1 us (4.7); backward 65536 x 192 31.8 us (4.7 TB/s), 8192 x 4096 78.6 us (5.1), each and then 8...9 us for the column
-// sums; 5003 x 1001 fp32 19.5, 26.9 and 7.8 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.7 us: a launch.
+// Measured (MI355X; a large copy reaches 5.0 TB/s here), bf16 unless noted: forward 262144 x 96 43.2 us (4.7 TB/s),
+// 65536 x 192 27.2 us (3.7), 8192 x 4096 RMS 57.0 us (4.7); backward 65536 x 192 30.3 us (5.0 TB/s), 8192 x 4096 77.8 us (5.2),
+// each followed by 8 us of column sums; 5003 x 1001 fp32 19.6, 26.8 and 7 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.6 us,
+// which is a launch and one pass through the loads.
 #include "unaligned.h"
 
 namespace {
@@ -378,7 +378,9 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
 
 // Sums of partials [rows][4][C] down the rows, in double, and the gradients made of them: blockIdx.y 0: the norm in front
 // (d0: weight, d1: bias), 1: gate, weight and bias of the norm behind (d2, d3, d4).  16 columns a workgroup, 32 row lanes a
-// sum with eight loads in flight each (a few MB that were just written: latency, not bytes).
+// sum with eight loads in flight each (a few MB that were just written: latency, not bytes; rows past the end load the last
+// one, since a condition would turn the eight into branches: the whole backward call at 65536 x 192 41.8 us with it, 37...40
+// without; 8 columns a workgroup take 8192 x 4096 from 87 to 93).
 struct SumArgs {
   float *d0, *d1, *d2, *d3, *d4;
   const float *gate, *post_w, *post_b;
@@ -394,9 +396,9 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
     for (int r0 = rl; r0 < rows; r0 += 32 * 8) {
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = r0 + 32 * j < rows ? p[(int64_t)(r0 + 32 * j) * 4 * C] : 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = p[(int64_t)min(r0 + 32 * j, rows - 1) * 4 * C];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t += (double)v[j];
+      for (int j = 0; j < 8; ++j) t += r0 + 32 * j < rows ? (double)v[j] : 0.0;
     }
   }
   red[which][rl][cl] = t;
