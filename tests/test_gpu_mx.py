@@ -298,3 +298,40 @@ def test_refusals():
         ops.mx_linear(y, qw)
     with torch.no_grad():
         ops.mx_linear(y, qw)
+
+
+def test_operands_that_share_memory():
+    from unet_amd import ops
+    for dt in (F32, BF):
+        qw, qn = ops.mx_quantize(make((96, 96), 2).cuda()), ops.mx_quantize(make((40, 96), 2).cuda())
+        wide = make((600, 200), 1, dt).cuda()
+        x, want = wide[:, :96], ops.mx_linear(wide[:, :96].contiguous(), qw)
+        assert torch.equal(ops.mx_linear(x, qw, out=wide[:, 96:192]), want)      # beside each other in one buffer
+        r = make((600, 40), 5, dt).cuda()
+        for out in (x, wide[:, 8:104], wide[:, 95:191]):
+            with pytest.raises(ValueError, match="shares memory with x"):
+                ops.mx_linear(x, qw, out=out)
+        buf = make((600, 64), 3, dt).cuda()
+        with pytest.raises(ValueError, match="without being resid"):
+            ops.mx_linear(x, qn, resid=buf[:, :40], out=buf[:, 8:48])
+        with pytest.raises(ValueError, match="without being resid"):
+            ops.mx_linear(x[1:], qn, resid=r[1:], out=r[:-1])
+        want = ops.mx_linear(x, qn, resid=r)
+        assert torch.equal(ops.mx_linear(x, qn, resid=r, out=r), want)
+
+
+def test_rows_beyond_32_bits():
+    """A wide row stride puts the last rows past 2^32 bytes, on either side."""
+    from unet_amd import ops
+    qw = ops.mx_quantize(make((72, 96), 2).cuda())
+    for rows, ld in ((20, 1 << 27), (600, 1 << 22)):
+        big = torch.empty(rows * ld, dtype=BF, device="cuda").view(rows, ld)
+        x = make((rows, 96), 1, BF).cuda()
+        big[:, :96] = x
+        want = ops.mx_linear(x, qw)
+        assert torch.equal(ops.mx_linear(big[:, :96], qw), want)
+        assert torch.equal(ops.mx_quantize(big[:, :96]).data, ops.mx_quantize(x).data)
+        big[:, 200:300] = 7
+        ops.mx_linear(x, qw, out=big[:, 208:280])
+        assert torch.equal(big[:, 208:280], want) and (big[:, 200:208] == 7).all() and (big[:, 280:300] == 7).all()
+        del big

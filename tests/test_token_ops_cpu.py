@@ -111,3 +111,22 @@ def test_steps_of_an_optimizer_are_known_to_its_parameters():
     two.step()
     two.step()
     assert (steps_taken(a), steps_taken(b)) == (3, 2)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5])
+def test_shared_memory_is_seen(rows):
+    """Against the set of bytes that each operand covers."""
+    for lda in (4, 6, 9):
+        for ldb in (4, 6, 9):
+            for ca in (1, 3, 4):
+                for cb in (1, 2, 4):
+                    for b in range(0, 60):
+                        a = 20
+                        one = {a + r * lda + c for r in range(rows) for c in range(ca)}
+                        two = {b + r * ldb + c for r in range(rows) for c in range(cb)}
+                        apart = ops._apart(a, ca, b, cb, rows, lda, ldb)
+                        if lda == ldb or rows == 1:
+                            # (one gap behind the last row may count as shared)
+                            assert apart <= (not one & two) and (apart or one & two or abs(b - a) <= rows * lda), (lda, ldb, ca, cb, b)
+                        else:
+                            assert apart <= (not one & two)

@@ -972,6 +972,15 @@ def _token_rows(t, what, device=None, dtype=None):
     return rows, ld
 
 
+def _apart(a, ca, b, cb, rows, lda, ldb):
+    """Whether no element of the ca columns from byte address a on is one of the cb from b on, rows of both lda and ldb
+    bytes apart (channel slices of one buffer may take turns in memory)."""
+    if a + (rows - 1) * lda + ca <= b or b + (rows - 1) * ldb + cb <= a:
+        return True
+    d = (b - a) % lda
+    return lda == ldb and d >= ca and d + cb <= lda
+
+
 def _vector(t, what, n, device):
     """Address of a contiguous float32 vector of n on device index ``device`` (None: null)."""
     if t is None:
@@ -1200,6 +1209,13 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
             ldo = _token_rows(out, "out", dev, dt)[1]
         if resid is not None:
             ldr = _token_rows(resid, "resid", dev, dt)[1]
+        if out is not None and rows and N:
+            e, to = dt.itemsize, out.data_ptr()
+            if not quantised and not _apart(x.data_ptr(), K * e, to, N * e, rows, ldx * e, ldo * e):
+                raise ValueError("mx_linear: out shares memory with x")
+            if resid is not None and not (resid.data_ptr() == to and ldr == ldo) and \
+                    not _apart(resid.data_ptr(), N * e, to, N * e, rows, ldr * e, ldo * e):
+                raise ValueError("mx_linear: out shares memory with resid without being resid")
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return mx_linear(x, w, bias, act, resid, out, dtype)
