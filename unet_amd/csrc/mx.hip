@@ -254,6 +254,72 @@ __device__ __forceinline__ void store_tile(const MxArgs& a, uint32_t m, uint32_t
   store8<T, ACT, WHOLE, 1>(a, m, n + 16, acc);
 }
 
+// Four vectors of each of a quad's lanes the other way round: v[k] of lane i <- v[i] of lane k
+template <int CTRL> __device__ __forceinline__ uint32_t quad_swap(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ void transpose_quad(u32x4 (&v)[4], int lane) {
+  const bool b0 = lane & 1, b1 = lane & 2;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {      // lanes 1 apart
+      const uint32_t lo = v[k][e], hi = v[k + 1][e], from_lo = quad_swap<0xB1>(lo), from_hi = quad_swap<0xB1>(hi);
+      v[k][e] = b0 ? from_hi : lo;
+      v[k + 1][e] = b0 ? hi : from_lo;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {      // 2 apart
+      const uint32_t lo = v[k][e], hi = v[k + 2][e], from_lo = quad_swap<0x4E>(lo), from_hi = quad_swap<0x4E>(hi);
+      v[k][e] = b1 ? from_hi : lo;
+      v[k + 2][e] = b1 ? hi : from_lo;
+    }
+  }
+}
+
+// 32 rows x 64 columns (c0, c1: the columns' halves), activation and no residual, in stores of 8 rows x 128 bytes: a quad
+// of lanes holds four rows' 16-byte pieces, and turned round each of its vectors is one row.  All lanes come here.
+template <typename T, bool ACT, bool WHOLE>
+__device__ __forceinline__ void store_rows(const MxArgs& a, uint32_t m0, uint32_t n0, int lane, const f32x16& c0, const f32x16& c1) {
+  constexpr int E = Vec16<T>::N;
+  const uint32_t m = m0 + frag_row(lane & 28), i = lane & 3, h = (lane >> 5) << 3;
+#pragma unroll
+  for (int part = 0; part < 8 / E; ++part) {      // (float: 128 bytes are 32 columns)
+    u32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x16& c = (E == 8 ? j >> 1 : part) ? c1 : c0;
+      const int at = E == 8 ? 8 * (j & 1) : 8 * (j >> 1) + 4 * (j & 1);
+      Vec16<T> o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = from_f32<T>(mx_act<T, ACT>(c[at + e]));
+      v[j] = __builtin_bit_cast(u32x4, o);
+      asm volatile("" : "+v"(v[j]));      // (one vector at a time: the registers are needed)
+    }
+    if (E == 8) {      // the lower half of the wave takes the left 32 columns, the upper half the right ones
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const auto t = __builtin_amdgcn_permlane32_swap(v[j][e], v[j + 2][e], false, false);
+          v[j][e] = t[0];
+          v[j + 2][e] = t[1];
+        }
+      const u32x4 t = v[1];
+      v[1] = v[2];
+      v[2] = t;
+    }
+    transpose_quad(v, lane);
+    const uint32_t n = n0 + (E == 8 ? 8 * i + 4 * h : 32 * part + 16 * (i >> 1) + 4 * (i & 1) + h);
+    const int left = (int)(a.N - n);              // (n may lie past the last column: below zero)
+    T* o = reinterpret_cast<T*>(a.out) + (int64_t)m * a.ldo + n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k, o += a.ldo)
+      if (m + k < a.M) store_part<WHOLE>(o, __builtin_bit_cast(Vec16<T>, v[k]), left);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // A wave's 64 x 64 tile in bfloat16 through LDS (TILE_LDS bytes of its own): stores of eight rows x 128 bytes instead of 32
 // rows x 32 bytes (8192^3: 295 us for the whole call, 313 without; in mx_rows_kernel the LDS it takes costs waves, and
 // 262144 x 96 -> 384 went from 66 to 87 us).  cWX: half W of the columns, half X of the rows.
@@ -327,18 +393,6 @@ struct Tile32 {
     acc[0] = mma32<1, 1>(w[1], x[1], acc[0], sw, sx);
   }
 };
-// 64 x 64, whole units: four fragments a step
-struct Tile64 {
-  static constexpr int SIDE = 64, NF = 4, NA = 16;
-  f32x16 acc[4];      // [columns' half][rows' half]
-  __device__ __forceinline__ void mma(const u32x4 (&w)[4], const u32x4 (&x)[4], uint32_t sw, uint32_t sx) {
-    static_for<8>([&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = decltype(ic)::value, kh = i >> 2, wf = i >> 1 & 1, xf = i & 1;
-      acc[wf * 2 + xf] = mma32<kh * 2 + wf, kh * 2 + xf>(w[kh * 2 + wf], x[kh * 2 + xf], acc[wf * 2 + xf], sw, sx);
-    });
-  }
-};
-
 template <typename T, typename SRC, typename TILE>
 __global__ __launch_bounds__(1024) void mx_split_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
@@ -505,7 +559,7 @@ __global__ __launch_bounds__(1024) void mx_split_kernel(MxArgs a) {
 // 384 -> 1152: 15.8 us (50 MB, 3.2 TB/s).  Stores past the caches (nontemporal) cost three times as much: the 32 bytes that
 // an instruction has of a row are no longer joined to lines.
 template <typename T, typename SRC, int KS>
-__global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
+__global__ __launch_bounds__(512, KS <= 2 ? 4 : KS <= 4 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
   typedef typename std::conditional<RAW, SRC, bf16>::type S;
   __shared__ u32x4 xl[KS][4][64];
@@ -568,28 +622,40 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : KS <= 3 ? 3 : 2) void mx_rows_ke
   __syncthreads();
 #pragma unroll 1
   for (uint32_t g = g0 + wave; g < g1; g += W) {
-    Tile64 t;
+    // (opaque: the addresses of all forms of the epilogue would otherwise be kept in registers across the loop)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    // 32 rows at a time, so that half the accumulators are alive
+    static_for<2>([&](auto xc) __attribute__((always_inline)) {
+      constexpr int x = decltype(xc)::value;
+      f32x16 acc[2];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const float* b = bias + (g - g0) * 64 + w * 32 + ((lane >> 5) << 3);
+      for (int w = 0; w < 2; ++w) {
+        const float* b = bias + (g - g0) * 64 + w * 32 + ((lane >> 5) << 3);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) t.acc[2 * w][i] = b[((i >> 3) << 4) + (i & 7)];
-      t.acc[2 * w + 1] = t.acc[2 * w];
-    }
+        for (int i = 0; i < 16; ++i) acc[w][i] = b[((i >> 3) << 4) + (i & 7)];
+      }
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const u32x4 xf[4] = {xl[k][0][lane], xl[k][1][lane], xl[k][2][lane], xl[k][3][lane]};
-      t.mma(wr[k], xf, ws[k], *reinterpret_cast<const uint32_t*>(&sl[k][lane][0]));
-      refill(g + W, k);
-    }
-    // (opaque: the compiler would otherwise move the multiplications in front of each row's store)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(t.acc[i]));
-    with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        store_tile<T, decltype(act)::value, decltype(whole)::value>(a, mg * 64 + (i & 1) * 32 + frag_row(lane & 31),
-                                                                    g * 64 + (i >> 1) * 32, lane, t.acc[i]);
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 x0 = xl[k][x][lane], x1 = xl[k][2 + x][lane];
+        const uint32_t sx = *reinterpret_cast<const uint32_t*>(&sl[k][lane][0]);
+        acc[0] = mma32<0, x>(wr[k][0], x0, acc[0], ws[k], sx);
+        acc[1] = mma32<1, x>(wr[k][1], x0, acc[1], ws[k], sx);
+        acc[0] = mma32<2, 2 + x>(wr[k][2], x1, acc[0], ws[k], sx);
+        acc[1] = mma32<3, 2 + x>(wr[k][3], x1, acc[1], ws[k], sx);
+        if constexpr (x == 1) refill(g + W, k);
+      }
+      // (opaque: the compiler would otherwise move the multiplications in front of each row's store)
+      asm volatile("" : "+v"(acc[0]), "+v"(acc[1]));
+      const uint32_t m = mg * 64 + x * 32;
+      with_epilogue(a, [&](auto act, auto whole) __attribute__((always_inline)) {
+        if (a.resid == nullptr) {
+          store_rows<T, decltype(act)::value, decltype(whole)::value>(a, m, g * 64, ln, acc[0], acc[1]);
+        } else {
+          store_tile<T, decltype(act)::value, decltype(whole)::value>(a, m + frag_row(ln & 31), g * 64, ln, acc[0]);
+          store_tile<T, decltype(act)::value, decltype(whole)::value>(a, m + frag_row(ln & 31), g * 64 + 32, ln, acc[1]);
+        }
+      });
     });
   }
 }
@@ -830,7 +896,7 @@ template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stre
   // group's results; 33 for 1 KB of weights), and the rounds of resident workgroups times a wave's own way through its
   // share.  (16384 x 384 -> 1152 is 15.8 us as picked; when it was 20.2, three waves and six splits, which has the fewer rounds,
   // took 25.9.)
-  const double ks = a.kt, resident = 256.0 * (a.kt == 1 ? 16 : a.kt <= 3 ? 12 : 8);
+  const double ks = a.kt, resident = 256.0 * (a.kt <= 2 ? 16 : a.kt <= 4 ? 12 : 8);
   uint32_t W = 4, splits = 1;
   double best = 1e30;
   const uint32_t s0 = (a.ngroups + 127) / 128;      // (at most 128 groups a workgroup: 32 KB of bias)
