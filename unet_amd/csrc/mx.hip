@@ -277,8 +277,9 @@ __device__ __forceinline__ void transpose_quad(u32x4 (&v)[4], int lane) {
   }
 }
 
-// 32 rows x 64 columns (c0, c1: the columns' halves), activation and no residual, in stores of 8 rows x 128 bytes: a quad
-// of lanes holds four rows' 16-byte pieces, and turned round each of its vectors is one row.  All lanes come here.
+// 32 rows x 64 columns (c0, c1: the columns' halves), activation and no residual, in stores whose quads of lanes write 64
+// consecutive bytes of a row: a quad holds four rows' 16-byte pieces, and turned round each of its vectors is one row's.
+// All lanes come here.
 template <typename T, bool ACT, bool WHOLE>
 __device__ __forceinline__ void store_rows(const MxArgs& a, uint32_t m0, uint32_t n0, int lane, const f32x16& c0, const f32x16& c1) {
   constexpr int E = Vec16<T>::N;
@@ -322,7 +323,7 @@ __device__ __forceinline__ void store_rows(const MxArgs& a, uint32_t m0, uint32_
 
 // A wave's 64 x 64 tile in bfloat16 through LDS (TILE_LDS bytes of its own): stores of eight rows x 128 bytes instead of 32
 // rows x 32 bytes (8192^3: 295 us for the whole call, 313 without; in mx_rows_kernel the LDS it takes costs waves, and
-// 262144 x 96 -> 384 went from 66 to 87 us).  cWX: half W of the columns, half X of the rows.
+// 262144 x 96 -> 384 went from 66 to 87 us when the results stayed in the last cache).  cWX: half W of the columns, half X of the rows.
 constexpr int TILE_LDS = 64 * 144;
 template <bool ACT, bool WHOLE>
 __device__ __forceinline__ void store_through_lds(const MxArgs& a, uint32_t m0, uint32_t n0, int lane, const f32x16& c00,
@@ -550,14 +551,13 @@ __global__ __launch_bounds__(1024) void mx_split_kernel(MxArgs a) {
   }
 }
 
-// ---- many rows, short K (KS steps of 128): a workgroup of W (two to eight) waves quantises 64 rows once into LDS and its
+// ---- many rows, short K (KS steps of 128): a workgroup of W (four or eight) waves quantises 64 rows once into LDS and its
 // waves take every W-th group of 64 columns.  The weights' fragments come straight from the caches into
 // a ring of registers, a group ahead; the rows' are read from LDS a step at a time.  Bound by the write of the output (a
 // store instruction whose lanes lie in many rows holds the CU's address path for some 100 cycles) and the arithmetic on it.
-// 262144 x 96 -> 384 with GELU: 61 us (45 without) into an output that stays in the last cache, 73 and 17 more until the
-// next kernel starts (the 32 MB in the L2 caches are written back then) into one that does not; a floor of 50.  16384 x
-// 384 -> 1152: 15.8 us (50 MB, 3.2 TB/s).  Stores past the caches (nontemporal) cost three times as much: the 32 bytes that
-// an instruction has of a row are no longer joined to lines.
+// 262144 x 96 -> 384 with GELU 75 us (252 MB, 3.4 TB/s, a floor of 50; 51 without GELU and with 288 columns); 16384 x 384 -> 1152
+// 15.1 us (50 MB, 3.3 TB/s).  With stores of 32 bytes in each of 32 rows the first took 90 us, 17 of them behind the
+// kernel's end, and 61 where the output stayed in the last cache; stores past the caches 204.
 template <typename T, typename SRC, int KS>
 __global__ __launch_bounds__(512, KS <= 2 ? 4 : KS <= 4 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
@@ -891,17 +891,17 @@ template <typename T, typename SRC> void launch_split_f(const MxArgs& a, hipStre
 template <typename T, typename SRC> void launch_rows(MxArgs& a, hipStream_t stream) {
   a.ngroups = (uint32_t)cdiv(a.N, 64);
   const uint32_t blocks = (uint32_t)cdiv(a.M, 64);
-  // How many waves share 64 rows, and over how many workgroups their columns are split, from what bounds the kernel, in
-  // cycles of a CU: its address path (about 100 for a load or store whose lanes lie in many rows: 16 of a step's rows, 8 of a
-  // group's results; 33 for 1 KB of weights), and the rounds of resident workgroups times a wave's own way through its
-  // share.  (16384 x 384 -> 1152 is 15.8 us as picked; when it was 20.2, three waves and six splits, which has the fewer rounds,
-  // took 25.9.)
+  // Whether four or eight waves share 64 rows (whole SIMDs: 65536 x 192 -> 576 26.9 us with four, 30.0 with five), and over how
+  // many workgroups their columns are split, from what bounds the kernel, in cycles of a CU: its address path (about 100 for
+  // a load or store whose lanes lie in many rows: 16 of a step's rows, 8 of a group's results; 33 for 1 KB of weights), and
+  // the rounds of resident workgroups times a wave's own way through its share.  (262144 x 96 -> 384 75.5 with four waves, 81.7 with
+  // eight; 16384 x 384 -> 1152 16.6 and 15.1; 4096 x 768 -> 2304 23.8 with eight, 16.6 split in two.)
   const double ks = a.kt, resident = 256.0 * (a.kt <= 2 ? 16 : a.kt <= 4 ? 12 : 8);
   uint32_t W = 4, splits = 1;
   double best = 1e30;
   const uint32_t s0 = (a.ngroups + 127) / 128;      // (at most 128 groups a workgroup: 32 KB of bias)
   for (uint32_t s = s0; s < s0 + 16 && s <= a.ngroups; ++s)
-    for (uint32_t w = 2; w <= 8; ++w) {
+    for (uint32_t w = 4; w <= 8; w += 4) {
       const uint32_t per = (a.ngroups + s - 1) / s, used = (a.ngroups + per - 1) / per;
       const double path = blocks * (used * ks * 1600.0 + a.ngroups * (800.0 + ks * 140.0)) / 256.0;
       const double rounds = (double)blocks * used * w / resident;
