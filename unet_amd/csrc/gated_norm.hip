@@ -15,7 +15,7 @@
 //
 // Measured (MI355X; a large copy reaches 5.0 TB/s here), bf16 unless noted: forward 262144 x 96 43.2 us (4.7 TB/s),
 // 65536 x 192 27.2 us (3.7), 8192 x 4096 RMS 57.0 us (4.7); backward 65536 x 192 30.3 us (5.0 TB/s), 8192 x 4096 77.8 us (5.2),
-// each followed by 8 us of column sums; 5003 x 1001 fp32 19.6, 26.8 and 7 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.6 us,
+// each followed by 5...8 us of column sums; 5003 x 1001 fp32 19.5, 26.6 and 6 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.6 us,
 // which is a launch and one pass through the loads.
 #include "unaligned.h"
 
