@@ -419,6 +419,11 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
                          int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
                          const float* pre_w, const float* pre_b, int rms, float eps, void* r, void* n, float* stats,
                          int64_t M, int C, int dtype, unetk_stream_t stream);
+/* The same with an eps for each of the two norms. */
+int unetk_gated_norm_fwd_eps(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
+                             int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                             const float* pre_w, const float* pre_b, int rms, float post_eps, float pre_eps, void* r, void* n,
+                             float* stats, int64_t M, int C, int dtype, unetk_stream_t stream);
 /* The gradients, from dr (of r; may be null when dn is not) and dn (of n; given exactly when pre_w is): dx, df, and
  * the parameters' (C floats each, null: not wanted; those of a parameter that is null have to be null).  stats: what
  * the forward pass left.  partials: unetk_gated_norm_bwd_rows(M, C) * 4 * C floats of scratch.  No atomics: the

@@ -1,0 +1,177 @@
+"""GPU tests of the gated norms, the 4-bit products and the SwinUNet options built on them, at the edges: norms with
+different eps, infinities and NaN, inputs that want a gradient, 4-bit weights whose parameters have changed.
+
+Tolerances are those of the operators' and the model's own tests: gated norms float32 5e-5 of the largest value (20e-5 for
+gradients: four times as many sums), bfloat16 2^-8 of the value more; float32 models 1e-4 relative L2, gradients 2e-2.
+Infinities and NaN have to stand where the definition in 64 bits has them.
+"""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from oracle import swin_oracle
+from oracle import weights as W
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def make(shape, seed, dt=F32, scale=1.0, mean=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g, dtype=torch.float64) * scale + mean).to(dt)
+
+
+def rel(a, b):
+    a, b = a.detach().double().cpu().reshape(-1), b.detach().double().cpu().reshape(-1)
+    return ((a - b).norm() / b.norm().clamp_min(1e-30)).item()
+
+
+def formula(x, f, dr, dn, gate=None, post=None, pre=None, kind="layer", post_eps=1e-5, pre_eps=1e-5):
+    """(r, n, gradients by name) in 64 bits; the gradients by autograd of the definition."""
+    lv = {}
+
+    def leaf(k, t):
+        if t is None:
+            return None
+        lv[k] = t.detach().double().cpu().requires_grad_(True)
+        return lv[k]
+
+    def normed(v, w, b, eps):
+        if kind == "layer":
+            v = v - v.mean(-1, keepdim=True)
+        v = v / torch.sqrt((v * v).mean(-1, keepdim=True) + eps) * w
+        return v if b is None else v + b
+    h = leaf("f", f)
+    X, g = leaf("x", x), leaf("gate", gate)
+    if post is not None:
+        h = normed(h, leaf("post_weight", post[0]), leaf("post_bias", post[1]), post_eps)
+    r = X + (h if g is None else h * g)
+    n = None if pre is None else normed(r, leaf("pre_weight", pre[0]), leaf("pre_bias", pre[1]), pre_eps)
+    outs = [t for t in (r, n) if t is not None]
+    grads = torch.autograd.grad(outs, list(lv.values()), [t.double().cpu() for t in (dr, dn) if t is not None])
+    return r.detach(), None if n is None else n.detach(), dict(zip(lv, grads))
+
+
+def agree(got, want, dt, what, extra=1.0):
+    """Equal infinities and NaN; finite values within the tolerance."""
+    got, want = got.detach().double().cpu(), want.detach().double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    assert torch.equal(torch.nan_to_num(got[~fin]), torch.nan_to_num(want[~fin])), what
+    big = want[fin].abs().max().clamp_min(1e-30)
+    tol = 5e-5 * extra * big + (2.0 ** -8 * want[fin].abs() if dt == BF else 0.0)
+    bad = ((got[fin] - want[fin]).abs() - tol).max().item()
+    assert bad <= 0, (what, bad, big.item())
+
+
+def check_norm(x, f, dr, dn, dt, names=None, rows=None, **kw):
+    """Both directions of the gated norm against the formula.  names: the gradients to look at (all of them), rows: which
+    rows of dx and df."""
+    from unet_amd import ops
+    cu = lambda t: None if t is None else t.cuda()
+    pair = lambda p: None if p is None else (cu(p[0]), cu(p[1]))
+    eps = (kw.get("post_eps", 1e-5), kw.get("pre_eps", 1e-5))
+    a = dict(gate=cu(kw.get("gate")), post=pair(kw.get("post")), pre=pair(kw.get("pre")), kind=kw.get("kind", "layer"),
+             eps=eps if eps[0] != eps[1] else eps[0])
+    r, n, st = ops.gated_norm_fwd(x.cuda(), f.cuda(), **a)
+    wr, wn, wg = formula(x, f, dr, dn, **kw)
+    agree(r, wr, dt, "r")
+    if wn is not None:
+        agree(n, wn, dt, "n")
+    got = ops.gated_norm_bwd(cu(dr), cu(dn), x.cuda(), f.cuda(), st, **a)
+    for name in got._fields:
+        t = getattr(got, name)
+        assert (t is None) == (name not in wg), name
+        if t is not None and (names is None or name in names):
+            of_rows = name in ("x", "f")
+            t, want = (v[rows] if of_rows and rows is not None else v for v in (t.cpu(), wg[name]))
+            agree(t, want, dt if of_rows else F32, name, 4.0)
+
+
+# ------------------------------------------------------------------ the two norms' eps
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("C", [77, 96, 1024])
+def test_each_norm_has_its_own_eps(C, dt, kind):
+    x, f = make((37, C), 1, dt, 0.3), make((37, C), 2, dt, 0.2)
+    for bias in (True, False):
+        vec = lambda s, m: make(C, s, F32, 0.2, m)
+        post, pre = (vec(3, 1.0), vec(4, 0.0) if bias else None), (vec(5, 1.0), vec(6, 0.0) if bias else None)
+        for pe, ne in ((0.25, 1e-5), (1e-5, 0.5), (0.1, 0.01), (0.03, 0.03)):
+            check_norm(x, f, make((37, C), 8, dt, 0.1), make((37, C), 9, dt, 0.1), dt, gate=vec(7, 0.5), post=post, pre=pre,
+                       kind=kind, post_eps=pe, pre_eps=ne)
+
+
+def norm_eps(name):
+    """An eps for a norm of a block: four different ones a block, others in the next."""
+    at = sum(int(c) for c in name if c.isdigit())
+    return (0.02, 0.3, 0.05, 0.11, 0.2)[(at + 2 * ("post" in name)) % 5]
+
+
+def gated_block(sd, pre, x, H, Wd, heads, ws, shift, mask, keep1=None, keep2=None):
+    """A block with norms behind its branches and gates, each norm with norm_eps of its name."""
+    B, L, C = x.shape
+    ln = lambda v, k: F.layer_norm(v, (C,), sd[pre + k + ".weight"], sd[pre + k + ".bias"], norm_eps(pre + k))
+
+    def branch(f, which, keep):
+        f = ln(f, f"post_norm{which}") * sd[pre + f"gate{which}"]
+        return f if keep is None else f * keep.view(B, 1, 1).to(f.dtype)
+    h = ln(x, "norm1").view(B, H, Wd, C)
+    He, We = max(H, ws), max(Wd, ws)
+    h = F.pad(h, (0, 0, 0, We - Wd, 0, He - H))
+    if shift > 0:
+        h = torch.roll(h, (-shift, -shift), (1, 2))
+    a = swin_oracle.window_attention(sd, pre + "attn.", swin_oracle._partition(h, ws), heads, ws,
+                                     None if mask is None else mask.to(x.dtype))
+    h = swin_oracle._unpartition(a, ws, He, We)
+    if shift > 0:
+        h = torch.roll(h, (shift, shift), (1, 2))
+    x = x + branch(h[:, :H, :Wd, :].reshape(B, L, C), 1, keep1)
+    y = F.linear(ln(x, "norm2"), sd[pre + "mlp.0.weight"], sd[pre + "mlp.0.bias"])
+    y = F.linear(F.gelu(y), sd[pre + "mlp.3.weight"], sd[pre + "mlp.3.bias"])
+    return x + branch(y, 2, keep2)
+
+
+def swin(dt, **options):
+    from unet_amd.swin import SwinUNet
+    cfg = dict(swin_oracle.DEFAULT_CONFIG, **options)
+    m = SwinUNet(cfg, compute_dtype=dt)
+    sd = W.fill_state_dict(swin_oracle.swin_template(cfg), seed=42)
+    for i, (k, v) in enumerate(m.state_dict().items()):
+        if k not in sd:
+            base = cfg["layer_scale"] if "gate" in k else 1.0 if k.endswith("weight") else 0.0
+            sd[k] = make(tuple(v.shape), 100 + i, F32, 0.2 * (base or 1.0), base)
+    m.load_state_dict(sd)
+    return m.cuda(), sd, cfg
+
+
+def test_a_gated_model_honours_every_norms_eps(monkeypatch):
+    monkeypatch.setattr(swin_oracle, "swin_block", gated_block)
+    m, sd, cfg = swin(F32, post_norm=True, layer_scale=0.5)
+    used = set()
+    for name, mod in m.named_modules():
+        if ".blocks." in name and isinstance(mod, torch.nn.LayerNorm):
+            mod.eps = norm_eps(name)
+            used.add((name.split(".")[1], name.split(".")[3], mod.eps))
+    assert sum(t[:2] == ("0", "0") for t in used) == 4      # four different ones in a block
+    x, y, _ = W.synthetic_batch(3, 4, 64, 64, seed=42)
+    assert rel(m.eval()(x.cuda()), swin_oracle.swin_unet_forward(sd, x, cfg, False)[0]) < 1e-4
+    m.train()
+    drop = [[None, None]] * sum(cfg["depths"])
+    m.drop_path_override = drop
+    out = m(x.cuda())
+    tgt = F.adaptive_avg_pool2d(y, out.shape[-2:])
+    ((out - tgt.cuda()) ** 2).mean().backward()
+    leaves = {k: v.double().requires_grad_(True) for k, v in sd.items() if v.is_floating_point() and "running_" not in k}
+    full = {k: leaves.get(k, v.double() if v.is_floating_point() else v) for k, v in sd.items()}
+    ref, _ = swin_oracle.swin_unet_forward(full, x.double(), cfg, True, drop)
+    ((ref - tgt.double()) ** 2).mean().backward()
+    assert rel(out, ref) < 1e-3      # (training mode: batch statistics over few elements)
+    got = dict(m.named_parameters())
+    num = sum(((got[k].grad.double().cpu() - t.grad) ** 2).sum() for k, t in leaves.items())
+    den = sum((t.grad ** 2).sum() for t in leaves.values())
+    assert (num / den).sqrt().item() < 2e-2
+    for k, t in leaves.items():
+        if ("gate" in k or "post_norm" in k or ".norm" in k) and t.grad.norm() > 1e-7 * den.sqrt():
+            assert rel(got[k].grad, t.grad) < 5e-2, k

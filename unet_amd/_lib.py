@@ -123,6 +123,7 @@ _SIGNATURES = {
     "unetk_dtable_reduce_batched": (I, [P, I, I, P]),
     "unetk_gated_norm_max_channels": (I, []),
     "unetk_gated_norm_fwd": (I, [P, L, P, L, P, P, L, F, P, P, P, P, I, F, P, P, P, L, I, I, P]),
+    "unetk_gated_norm_fwd_eps": (I, [P, L, P, L, P, P, L, F, P, P, P, P, I, F, F, P, P, P, L, I, I, P]),
     "unetk_gated_norm_bwd_rows": (I, [L, I]),
     "unetk_gated_norm_bwd": (I, [P, L, P, L, P, L, P, L, P, P, P, L, F, P, P, P, I, P, P, P, P, P, P, P, P, L, I, I, P]),
     "unetk_mx_codes_bytes": (L, [L, L]),

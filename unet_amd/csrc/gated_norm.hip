@@ -35,7 +35,7 @@ struct NormArgs {
   float* partials;       // [workgroups][4][C]
   uint32_t M, rps;       // rows; rows per sample
   int C, rms;
-  float res_scale, eps;
+  float res_scale, post_eps, pre_eps;
 };
 
 // The elements of a row that one of its G lanes holds: N = NV 16-byte vectors, at whatever address the row begins.
@@ -144,8 +144,8 @@ template <int G> struct RowSum {
 // mean (0 for RMSNorm) and 1 / sqrt(mean square distance from it + eps) of the row whose elements the lanes hold: from
 // registers, in two passes, so that rows far from zero keep their digits
 template <typename L, int G>
-__device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], RowSum<G>& rs, const NormArgs& a, float inv_c,
-                                        float& mean, float& rstd) {
+__device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], RowSum<G>& rs, const NormArgs& a, float eps,
+                                        float inv_c, float& mean, float& rstd) {
   mean = 0.f;
   if (!a.rms) {
     float s = 0.f;
@@ -159,7 +159,7 @@ __device__ __forceinline__ void moments(const L& ln, const float (&v)[L::N], Row
     const float d = ln.has(i) ? v[i] - mean : 0.f;
     q += d * d;
   }
-  rstd = 1.0f / sqrtf(rs.sum(q) * inv_c + a.eps);
+  rstd = 1.0f / sqrtf(rs.sum(q) * inv_c + eps);
 }
 
 // One element of r, in the operations that both directions use (explicit fused multiply-adds: whatever the compiler
@@ -211,14 +211,14 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
     float fm = 0.f, fs = 0.f, rm = 0.f, rsd = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) h[i] = L::at(fr, i);
-    if (post) moments(ln, h, rs, a, inv_c, fm, fs);
+    if (post) moments(ln, h, rs, a, a.post_eps, inv_c, fm, fs);
     const float hs = post ? fs : 1.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
       r[i] = ln.has(i) ? residual(L::at(xr, i), norm_hat(h[i], fm, hs), qw[i], qb[i], keep, a.res_scale) : 0.f;
     if (live) ln.store(reinterpret_cast<T*>(a.o0) + (int64_t)row * a.C, r);
     if (pre) {
-      moments(ln, r, rs, a, inv_c, rm, rsd);
+      moments(ln, r, rs, a, a.pre_eps, inv_c, rm, rsd);
 #pragma unroll
       for (int i = 0; i < N; ++i) r[i] = norm_hat(r[i], rm, rsd) * pw[i] + pb[i];
       if (live) ln.store(reinterpret_cast<T*>(a.o1) + (int64_t)row * a.C, r);
@@ -483,10 +483,10 @@ extern "C" {
 
 int unetk_gated_norm_max_channels(void) { return NORM_MAX_C; }
 
-int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
-                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
-                         const float* pre_w, const float* pre_b, int rms, float eps, void* r, void* n, float* stats,
-                         int64_t M, int C, int dtype, hipStream_t stream) {
+int unetk_gated_norm_fwd_eps(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
+                             int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                             const float* pre_w, const float* pre_b, int rms, float post_eps, float pre_eps, void* r, void* n,
+                             float* stats, int64_t M, int C, int dtype, hipStream_t stream) {
   const int rc = check_norm("gated_norm_fwd", M, C, dtype, keep, rows_per_sample);
   if (rc != UNETK_OK) return rc;
   UNETK_CHECK_ARG(x && f && r && ldx >= C && ldf >= C, "gated_norm_fwd: null operand or overlapping rows");
@@ -495,7 +495,8 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
   NormArgs a = {};
   a.x = x; a.f = f; a.ldx = ldx; a.ldf = ldf; a.gate = gate; a.keep = keep; a.post_w = post_w; a.post_b = post_b;
   a.pre_w = pre_w; a.pre_b = pre_b; a.stats_out = stats; a.o0 = r; a.o1 = n; a.M = (uint32_t)M;
-  a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms; a.res_scale = res_scale; a.eps = eps;
+  a.rps = keep ? (uint32_t)rows_per_sample : 1; a.C = C; a.rms = rms; a.res_scale = res_scale;
+  a.post_eps = post_eps; a.pre_eps = pre_eps;
   const bool whole = C % (dtype == UNETK_BF16 ? 8 : 4) == 0;
   // about what the chip holds at once, so that a workgroup has many rows to fetch ahead over (262144 x 96: 43.2 us with
   // 1536, 50.1 with 4096; 8192 x 4096: 47.9 with 1024, 49.1 with 1536, 53.4 with 4096)
@@ -504,6 +505,14 @@ int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf,
   else NORM_DISPATCH(gated_norm_fwd_kernel, float);
   UNETK_CHECK_LAUNCH();
   return UNETK_OK;
+}
+
+int unetk_gated_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const float* gate, const float* keep,
+                         int64_t rows_per_sample, float res_scale, const float* post_w, const float* post_b,
+                         const float* pre_w, const float* pre_b, int rms, float eps, void* r, void* n, float* stats,
+                         int64_t M, int C, int dtype, hipStream_t stream) {
+  return unetk_gated_norm_fwd_eps(x, ldx, f, ldf, gate, keep, rows_per_sample, res_scale, post_w, post_b, pre_w, pre_b, rms, eps,
+                                  eps, r, n, stats, M, C, dtype, stream);
 }
 
 int unetk_gated_norm_bwd_rows(int64_t M, int C) {

@@ -1046,11 +1046,12 @@ def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=Non
 
     x: the residual stream, f: the branch's output, (..., C) float32 or bfloat16 with equally spaced rows (dense, or a
     channel slice).  post, pre: (weight, bias or None) of the two norms, each may be None; kind: "layer" or "rms" (without
-    the mean).  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
+    the mean); eps: under both norms' roots, or a pair of them, post's and pre's.  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
     float32.  Returns (r, n, stats): r and n dense, n None without pre; stats is what gated_norm_bwd reads (None unless
     want_stats).  n is taken from the unrounded r."""
     a_keep = keep
     M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
+    post_eps, pre_eps = eps if isinstance(eps, (tuple, list)) else (eps, eps)
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return gated_norm_fwd(x, f, gate, a_keep, res_scale, post, pre, kind, eps, want_stats)
@@ -1058,8 +1059,8 @@ def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=Non
     n = torch.empty_like(r) if pw is not None else None
     stats = torch.empty((M, 4), dtype=torch.float32, device=x.device) if want_stats else None
     if M:
-        call("unetk_gated_norm_fwd", x.data_ptr(), ldx, f.data_ptr(), ldf, g, keep, rps, res_scale, qw, qb, pw, pb,
-             kind == "rms", eps, r.data_ptr(), _at(n), _at(stats), M, C, code, stream())
+        call("unetk_gated_norm_fwd_eps", x.data_ptr(), ldx, f.data_ptr(), ldf, g, keep, rps, res_scale, qw, qb, pw, pb,
+             kind == "rms", post_eps, pre_eps, r.data_ptr(), _at(n), _at(stats), M, C, code, stream())
     return r, n, stats
 
 

@@ -614,9 +614,10 @@ def _norm_of(norm):
 
 def _gated_args(blk, which, nxt):
     """Arguments of ops.gated_norm_fwd / _bwd at the end of a block's branch: its gate and the norm behind it, and the norm
-    in front of what follows."""
+    in front of what follows, each norm with its own eps."""
     gate, post = (blk.gate1, blk.post_norm1) if which == 1 else (blk.gate2, blk.post_norm2)
-    return dict(gate=gate, post=_norm_of(post), pre=_norm_of(nxt), eps=blk.norm1.eps)
+    eps = tuple(0.0 if norm is None else norm.eps for norm in (post, nxt))
+    return dict(gate=gate, post=_norm_of(post), pre=_norm_of(nxt), eps=eps)
 
 
 def _gated_block_fwd(blk, pre, x, ln1, keep1, keep2, cx, save, nxt):
