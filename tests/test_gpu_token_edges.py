@@ -175,3 +175,19 @@ def test_a_gated_model_honours_every_norms_eps(monkeypatch):
     for k, t in leaves.items():
         if ("gate" in k or "post_norm" in k or ".norm" in k) and t.grad.norm() > 1e-7 * den.sqrt():
             assert rel(got[k].grad, t.grad) < 5e-2, k
+
+
+# ------------------------------------------------------------------ infinities and NaN
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("C", [77, 96, 4096])
+def test_an_infinite_column_sum_stays_infinite_without_a_bias(C, kind):
+    """dgate = w sum(u fhat) + b sum(u): without b there is no second term, and infinity times nothing is not NaN."""
+    x, f, dr = make((40, C), 1), make((40, C), 2), make((40, C), 3)
+    dr[7, 5], dr[20, C - 1] = float("inf"), float("-inf")
+    w, gate = make(C, 4, F32, 0.2, 1.0), make(C, 5, F32, 0.2, 0.5)
+    want = formula(x, f, dr, None, gate=gate, post=(w, None), kind=kind)[2]
+    assert torch.isinf(want["gate"]).sum() == 2 and torch.isinf(want["post_weight"]).sum() == 2
+    # (behind a norm the two rows' own gradients are infinities added and subtracted: what of them is NaN is no one's)
+    rows = [i for i in range(40) if i not in (7, 20)]
+    check_norm(x, f, dr, None, F32, rows=rows, gate=gate, post=(w, None), kind=kind)
+    check_norm(x, f, dr, None, F32, gate=gate, kind=kind)

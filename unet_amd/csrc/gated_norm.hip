@@ -417,7 +417,11 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* __restri
       if (o.d1) o.d1[col] = (float)other;
     } else {
       const double gate = o.gate ? (double)o.gate[col] : 1.0;
-      if (o.d2) o.d2[col] = (float)(t * (o.post_w ? (double)o.post_w[col] : 1.0) + other * (o.post_b ? (double)o.post_b[col] : 0.0));
+      if (o.d2) {      // (an absent bias adds no term: a sum may be infinite, and infinity times zero is NaN)
+        double d = t * (o.post_w ? (double)o.post_w[col] : 1.0);
+        if (o.post_b) d += other * (double)o.post_b[col];
+        o.d2[col] = (float)d;
+      }
       if (o.d3) o.d3[col] = (float)(gate * t);
       if (o.d4) o.d4[col] = (float)(gate * other);
     }
