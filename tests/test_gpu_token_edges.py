@@ -191,3 +191,16 @@ def test_an_infinite_column_sum_stays_infinite_without_a_bias(C, kind):
     rows = [i for i in range(40) if i not in (7, 20)]
     check_norm(x, f, dr, None, F32, rows=rows, gate=gate, post=(w, None), kind=kind)
     check_norm(x, f, dr, None, F32, gate=gate, kind=kind)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("C", [77, 96, 8192])
+def test_an_infinite_gate_without_a_bias_behind_it(C, dt):
+    x, f, dr = make((5, C), 1, dt), make((5, C), 2, dt), make((5, C), 3, dt)
+    w, gate = make(C, 4, F32, 0.2, 1.0), make(C, 5, F32, 0.2, 0.5)
+    gate[3], gate[C - 1] = float("inf"), float("-inf")
+    assert torch.isinf(formula(x, f, dr, None, gate=gate)[0]).sum() == 10
+    check_norm(x, f, dr, None, dt, gate=gate)
+    # (infinities of both signs are added up in what flows back through a norm)
+    check_norm(x, f, dr, None, dt, names=("x", "gate"), gate=gate, post=(w, None))
+    check_norm(x, f, dr, make((5, C), 6, dt), dt, names=(), gate=gate, pre=(w, None), kind="rms")

@@ -180,7 +180,8 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
   const uint32_t rg = threadIdx.x / G;
   const float inv_c = 1.0f / (float)a.C;
   const bool post = a.post_w != nullptr, pre = a.pre_w != nullptr;
-  // gate * (fhat * w_post + b_post) = fhat * (gate w_post) + gate b_post
+  // gate * (fhat * w_post + b_post) = fhat * (gate w_post) + gate b_post, the second term 0 without a bias (a gate may be
+  // infinite, and infinity times zero is NaN)
   float qw[N], qb[N], pw[N], pb[N];
   {
     float gate[N];
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_fwd_kernel(NormArgs 
     ln.param(qw, a.post_w, 1.f);
     ln.param(qb, a.post_b, 0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) qw[i] *= gate[i], qb[i] *= gate[i];
+    for (int i = 0; i < N; ++i) qw[i] *= gate[i], qb[i] = a.post_b != nullptr ? qb[i] * gate[i] : 0.f;
   }
   ln.param(pw, a.pre_w, 1.f);
   ln.param(pb, a.pre_b, 0.f);
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
     put(0, w);
     ln.param(w, a.post_b, 0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] *= gate[i];
+    for (int i = 0; i < N; ++i) w[i] = a.post_b != nullptr ? w[i] * gate[i] : 0.f;
     put(1, w);
     ln.param(w, a.pre_w, 0.f);
     put(2, w);
