@@ -204,3 +204,33 @@ def test_an_infinite_gate_without_a_bias_behind_it(C, dt):
     # (infinities of both signs are added up in what flows back through a norm)
     check_norm(x, f, dr, None, dt, names=("x", "gate"), gate=gate, post=(w, None))
     check_norm(x, f, dr, make((5, C), 6, dt), dt, names=(), gate=gate, pre=(w, None), kind="rms")
+
+
+@pytest.mark.parametrize("M", [1, 3, 17, 63])
+@pytest.mark.parametrize("C", [24, 96, 200])
+def test_an_infinite_last_row_counts_once(M, C):
+    """Workgroups of several rows, the last of them short: the rows that are not there add nothing, whatever the last holds."""
+    x, f, dr = make((M, C), 1), make((M, C), 2), make((M, C), 3).abs()
+    f[M - 1, 2], f[M - 1, C - 1] = float("inf"), float("-inf")
+    gate = make(C, 5, F32, 0.2, 0.5)
+    assert torch.isinf(formula(x, f, dr, None, gate=gate)[2]["gate"]).sum() == 2
+    check_norm(x, f, dr, None, F32, gate=gate)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("C", [77, 96, 512])
+def test_nan_and_infinite_rows_stay_alone(C, dt):
+    from unet_amd import ops
+    x, f, dr, dn = (make((70, C), i, dt) for i in range(4))
+    f[69, 0], x[3, C - 1], f[40, 5], dr[50, 1] = float("nan"), float("inf"), float("-inf"), float("nan")
+    w, b, gate = make(C, 4, F32, 0.2, 1.0).cuda(), make(C, 6).cuda(), make(C, 5, F32, 0.2, 0.5).cuda()
+    kw = dict(gate=gate, post=(w, b), pre=(w, b))
+    r, n, st = ops.gated_norm_fwd(x.cuda(), f.cuda(), **kw)
+    assert (~torch.isfinite(n)).any(1).nonzero().flatten().tolist() == [3, 40, 69]
+    assert (~torch.isfinite(r)).any(1).nonzero().flatten().tolist() == [3, 40, 69]
+    d = ops.gated_norm_bwd(dr.cuda(), dn.cuda(), x.cuda(), f.cuda(), st, **kw)
+    for t in (d.x, d.f):
+        assert (~torch.isfinite(t)).any(1).nonzero().flatten().tolist() == [3, 40, 50, 69]
+    keep = [i for i in range(70) if i not in (3, 40, 50, 69)]
+    y = ops.gated_norm_bwd(dr[keep].cuda(), dn[keep].cuda(), x[keep].cuda(), f[keep].cuda(), st[keep].contiguous(), **kw)
+    assert torch.equal(d.x[keep], y.x) and torch.equal(d.f[keep], y.f)

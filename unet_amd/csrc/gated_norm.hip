@@ -302,7 +302,7 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
   const uint32_t step = gridDim.x * RPB;
   if (blockIdx.x * RPB < a.M) fetch(blockIdx.x * RPB);
   for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += step) {
-    const bool live = row0 + rg < a.M;
+    const bool live = RPB == 1 || row0 + rg < a.M;
     const uint32_t row = live ? row0 + rg : row0;
     const typename L::Raw xr = nx.x, fr = nx.f, dr = nx.dr, dn = nx.dn;
     const f32x4 st = nx.st;
@@ -337,7 +337,8 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f, fh = norm_hat(L::at(fr, i), fm, fs);
+      // (lanes past the last row hold its values again: zero times an infinite one would be NaN)
+      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f, fh = live ? norm_hat(L::at(fr, i), fm, fs) : 0.f;
       acc[2][i] += u * fh;
       acc[3][i] += u;
       o[i] = u * prm(0, i);
