@@ -234,3 +234,18 @@ def test_nan_and_infinite_rows_stay_alone(C, dt):
     keep = [i for i in range(70) if i not in (3, 40, 50, 69)]
     y = ops.gated_norm_bwd(dr[keep].cuda(), dn[keep].cuda(), x[keep].cuda(), f[keep].cuda(), st[keep].contiguous(), **kw)
     assert torch.equal(d.x[keep], y.x) and torch.equal(d.f[keep], y.f)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("rows,K,N", [(20, 300, 40), (600, 1000, 700), (1100, 200, 130), (3400, 900, 3100)])
+def test_gelu_of_infinities(rows, K, N, dt):
+    """v Phi(v) at -infinity is infinity times nothing: NaN, in either type and every kernel; +infinity stays, and a large
+    negative number is nothing."""
+    from unet_amd import ops
+    x, qw, bias = make((rows, K), 1, dt).cuda(), ops.mx_quantize(make((N, K), 2, F32, K ** -0.5).cuda()), make(N, 3).cuda()
+    plain = ops.mx_linear(x, qw, bias=bias, act=2)
+    bias[1], bias[N - 1], bias[5] = float("-inf"), float("inf"), -3e38
+    y = ops.mx_linear(x, qw, bias=bias, act=2)
+    assert torch.isnan(y[:, 1]).all() and (y[:, N - 1] == float("inf")).all() and (y[:, 5].abs() < 1e-6).all()
+    rest = [i for i in range(N) if i not in (1, 5, N - 1)]
+    assert torch.equal(y[:, rest], plain[:, rest])

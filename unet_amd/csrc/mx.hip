@@ -193,7 +193,8 @@ __device__ __forceinline__ f32x4 mma16(const u32x4& w, const u32x4& x, f32x4 c, 
 // a polynomial of degree 6 in a suffices: the result is off by less than 2.4e-7 of v, and by less than 1.6e-4 of itself
 // far into the tail (least squares in the Chebyshev basis on [0, 5.5], reweighted towards the largest error against those
 // two; Phi(-5.5) = 2e-8 stands for what lies beyond).  Seven multiply-adds and one exponential instead of the erf form's
-// reciprocal, exponential and more.  NaN and +infinity pass through the first term.
+// reciprocal, exponential and more.  The first term is v / 2 + |v| / 2, exact for normal numbers: NaN and +infinity pass
+// through it, and -infinity makes it NaN, as the erf form does (infinity times zero).
 __device__ __forceinline__ float gelu_bf16(float v) {
   const float a = __builtin_amdgcn_fmed3f(fabsf(v), 0.f, 5.5f);
   float p = 3.13768651e-05f;
@@ -203,7 +204,7 @@ __device__ __forceinline__ float gelu_bf16(float v) {
   p = fmaf(p, a, -0.458968848f);
   p = fmaf(p, a, -1.15113544f);
   p = fmaf(p, a, -0.999999404f);
-  return fmaf(-a, __builtin_amdgcn_exp2f(p), v < 0.f ? 0.f : v);
+  return fmaf(-a, __builtin_amdgcn_exp2f(p), fmaf(0.5f, fabsf(v), 0.5f * v));
 }
 
 template <typename T, bool GELU> __device__ __forceinline__ float mx_act(float v) {
