@@ -249,3 +249,26 @@ def test_gelu_of_infinities(rows, K, N, dt):
     assert torch.isnan(y[:, 1]).all() and (y[:, N - 1] == float("inf")).all() and (y[:, 5].abs() < 1e-6).all()
     rest = [i for i in range(N) if i not in (1, 5, N - 1)]
     assert torch.equal(y[:, rest], plain[:, rest])
+
+
+# ------------------------------------------------------------------ inputs that want a gradient
+def test_4_bit_operators_refuse_what_wants_a_gradient():
+    from unet_amd import ops
+    for dt in (F32, BF):
+        x, w, b = make((6, 96), 1, dt).cuda(), make((40, 96), 2).cuda(), make(40, 3).cuda()
+        res, out = make((6, 40), 4, dt).cuda(), torch.empty((6, 40), dtype=dt, device="cuda")
+        qw, qx = ops.mx_quantize(w), ops.mx_quantize(x)
+        want = ops.mx_linear(x, qw, bias=b, resid=res)
+        leaf = lambda t: t.detach().clone().requires_grad_(True)
+        calls = [lambda: ops.mx_linear(leaf(x), qw, bias=b, resid=res), lambda: ops.mx_linear(x, qw, bias=leaf(b), resid=res),
+                 lambda: ops.mx_linear(x, qw, bias=b, resid=leaf(res)), lambda: ops.mx_linear(qx, qw, bias=b, resid=leaf(res), dtype=dt),
+                 lambda: ops.mx_linear(qx, qw, bias=leaf(b), resid=res, dtype=dt),
+                 lambda: ops.mx_linear(x, qw, bias=b, resid=res, out=leaf(out)),
+                 lambda: ops.mx_linear(x, ops.mx_quantize(leaf(w)), bias=b, resid=res),
+                 lambda: ops.mx_linear(ops.mx_quantize(leaf(x)), qw, bias=b, resid=res, dtype=dt)]
+        for i, f in enumerate(calls):
+            with pytest.raises(RuntimeError, match="gradient"):
+                f()
+                pytest.fail(f"call {i} was not refused")
+            with torch.no_grad():
+                assert torch.equal(f(), want), i

@@ -1116,6 +1116,14 @@ def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, pos
     return GatedNormGrads(dx, df, dg, dqw, dqb, dpw, dpb)
 
 
+def _no_gradient(what, *tensors):
+    """Refuses inputs (None: not given) that want a gradient: autograd does not see the call, and theirs would be lost."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach its inputs")
+
+
 class MxTensor:
     """A (..., K) tensor in microscaled 4-bit floating point (OCP MXFP4): blocks of 32 along K, E2M1 elements and one
     power-of-two scale a block, in the order in which the matrix instruction reads them.  Made by mx_quantize; read by
@@ -1138,8 +1146,10 @@ class MxTensor:
 def mx_quantize(x) -> MxTensor:
     """x (..., K), float32 or bfloat16 with equally spaced rows, in 4 bits: per block of 32 along K the scale
     2^(floor(log2 max) - 2) and the elements rounded half to even to 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (larger ones:
-    6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros."""
+    6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros.  It has no
+    gradient, and refuses an x that wants one."""
     rows, ld = _token_rows(x, "x")
+    _no_gradient("mx_quantize", x)
     code, K, dev = dtype_code(x.dtype), x.shape[-1], x.get_device()
     if K < 1:
         raise ValueError("mx_quantize: no elements to scale (K = 0)")
@@ -1173,10 +1183,11 @@ def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:
 
 def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None):
     """act(x @ w^T + bias) + resid with both operands in microscaled 4 bits and fp32 sums; for prediction (it has no
-    gradient).  x (..., K): a float32 or bfloat16 tensor, quantised on the way, or an MxTensor (quantised once for
-    several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none, 2 GELU (erf form);
-    resid: (..., N) of the result's type.  The result has x's type (``dtype`` for an MxTensor, bfloat16 if not given); out:
-    a (..., N) tensor or channel slice to write it to (it may be resid itself, but share no memory with x)."""
+    gradient, and refuses inputs that want one).  x (..., K): a float32 or bfloat16 tensor, quantised on the way, or an
+    MxTensor (quantised once for several products); w: mx_quantize of the (N, K) weight.  bias: (N,) float32; act: 0 none,
+    2 GELU (erf form); resid: (..., N) of the result's type.  The result has x's type (``dtype`` for an MxTensor, bfloat16
+    if not given); out: a (..., N) tensor or channel slice to write it to (it may be resid itself, but share no memory with
+    x)."""
     if not isinstance(w, MxTensor) or len(w.shape) != 2:
         raise TypeError("mx_linear: w is mx_quantize of the (N, K) weight")
     N, K = w.shape
@@ -1191,8 +1202,6 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
         dt = x.dtype
         if dtype is not None and dtype != dt:
             raise ValueError(f"mx_linear: dtype {dtype} for x of {dt}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("mx_linear has no gradient: call it under torch.no_grad(), or detach x")
     shape = x.shape
     if len(shape) < 1 or shape[-1] != K:
         raise ValueError(f"mx_linear: x {tuple(shape)} against w {tuple(w.shape)}")
@@ -1217,6 +1226,7 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
             if resid is not None and not (resid.data_ptr() == to and ldr == ldo) and \
                     not _apart(resid.data_ptr(), N * e, to, N * e, rows, ldr * e, ldo * e):
                 raise ValueError("mx_linear: out shares memory with resid without being resid")
+    _no_gradient("mx_linear", None if quantised else x, bias, resid, out)
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return mx_linear(x, w, bias, act, resid, out, dtype)
