@@ -272,3 +272,43 @@ def test_4_bit_operators_refuse_what_wants_a_gradient():
                 pytest.fail(f"call {i} was not refused")
             with torch.no_grad():
                 assert torch.equal(f(), want), i
+
+
+# ------------------------------------------------------------------ 4-bit weights whose parameters have changed
+def quantised_model(dt=BF, **options):
+    m, sd, cfg = swin(dt, **options)
+    x = W.synthetic_batch(1, 4, 64, 64, seed=42)[0].cuda()
+    m.eval().quantize_linears()
+    return m, x
+
+
+def replace_by_loading(m):
+    m.load_state_dict({k: v * 1.5 if v.is_floating_point() else v for k, v in m.state_dict().items()}, assign=True)
+
+
+def replace_parameter(m):
+    w = m.layers[0].blocks[1].mlp[0].weight
+    m.layers[0].blocks[1].mlp[0].weight = torch.nn.Parameter(w.detach() * 1.5)
+
+
+def replace_module(m):
+    old = m.layers[1].blocks[0].attn.proj
+    m.layers[1].blocks[0].attn.proj = torch.nn.Linear(old.in_features, old.out_features).to(old.weight.device)
+
+
+def replace_block(m):
+    from unet_amd.swin import SwinTransformerBlock
+    b = m.layers[1].blocks[0]
+    m.layers[1].blocks[0] = SwinTransformerBlock(b.dim, b.num_heads, b.window_size, b.shift_size, b.mlp_ratio).cuda().eval()
+
+
+@pytest.mark.parametrize("change", [replace_by_loading, replace_parameter, replace_module, replace_block])
+def test_replaced_parameters_are_refused_until_quantised_again(change):
+    m, x = quantised_model()
+    with torch.no_grad():
+        a = m(x)
+        change(m)
+        with pytest.raises(RuntimeError, match="quantize_linears"):
+            m(x)
+        assert not torch.equal(m.quantize_linears()(x), a)
+        assert torch.equal(m(x), m(x))

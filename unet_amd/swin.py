@@ -176,7 +176,7 @@ class SwinUNet(nn.Module):
         self.drop_path_override: Optional[List] = None
         # data-parallel hook, see unet_amd.dist.GradReducer
         self.grad_sink = None
-        self._mx_linears = None         # quantize_linears()
+        self._mx_linears = self._mx_links = None         # quantize_linears()
 
     def _init_weights(self, m):
         # reference swin_unet_model.py:616-630 (ConvTranspose2d is not a Conv2d: keeps its default init)
@@ -196,22 +196,32 @@ class SwinUNet(nn.Module):
         """Prediction with the token linears (qkv, proj, fc1, fc2, patch merging) in microscaled 4 bits: their weights are
         quantised now and kept beside the parameters, their inputs on the way (ops.mx_linear).  Eval mode only: training
         steps use the parameters themselves.  A forward pass in eval mode raises once a quantised parameter has been
-        changed or moved; call this again (or dequantize_linears()) after that.  (Seen are changes that count in autograd's
-        version counter, and FusedAdamW's steps, replayed ones too; not writes through ``parameter.data``.)  Returns self."""
-        weights = []
-        for layer in self.layers:
-            for blk in layer.blocks:
-                weights += [blk.attn.qkv.weight, blk.attn.proj.weight, blk.mlp[0].weight, blk.mlp[3].weight]
+        changed, moved or replaced; call this again (or dequantize_linears()) after that.  (Seen are changes that count in
+        autograd's version counter, FusedAdamW's steps, replayed ones too, and another parameter or module in the place of
+        one that was there; not writes through ``parameter.data``.)  Returns self."""
+        names = []
+        for li, layer in enumerate(self.layers):
+            for bi in range(len(layer.blocks)):
+                names += [f"layers.{li}.blocks.{bi}.{n}.weight" for n in ("attn.qkv", "attn.proj", "mlp.0", "mlp.3")]
             if layer.downsample is not None:
-                weights.append(layer.downsample.reduction.weight)
+                names.append(f"layers.{li}.downsample.reduction.weight")
+        weights, links = [], {}
+        for name in names:
+            at = self
+            for part in name.split("."):      # where each module and parameter on the way hangs, to see it replaced
+                table = at._parameters if part in at._parameters else at._modules
+                at = table[part]
+                links[id(table), part] = (table, part, at)
+            weights.append(at)
         if not all(w.is_cuda for w in weights):
             raise RuntimeError("quantize_linears: move the model to the GPU first")
+        self._mx_links = list(links.values())
         self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), (w._version, steps_taken(w))) for w in weights]
         return self
 
     def dequantize_linears(self):
         """Back to the parameters themselves in eval mode.  Returns self."""
-        self._mx_linears = None
+        self._mx_linears = self._mx_links = None
         return self
 
     def late_grad_names(self):
@@ -294,10 +304,11 @@ class _Ctx:
         held = getattr(model, "_mx_linears", None)
         if held is not None and not training:
             self.mx = {}
+            changed = any(table.get(part) is not was for table, part, was in model._mx_links)
             for w, q, at, version in held:
-                if w.data_ptr() != at or (w._version, steps_taken(w)) != version:
-                    raise RuntimeError("a SwinUNet parameter was changed or moved after quantize_linears(): call it again, "
-                                       "or dequantize_linears()")
+                if changed or w.data_ptr() != at or (w._version, steps_taken(w)) != version:
+                    raise RuntimeError("a SwinUNet parameter was changed, moved or replaced after quantize_linears(): call it "
+                                       "again, or dequantize_linears()")
                 self.mx[at] = q
         # (the walk over the module tree costs the host ~1 ms: its result is kept on the model, which does not
         # grow layers between steps; what can change - device, dtype, layout of a weight - is checked every time)
