@@ -312,3 +312,37 @@ def test_replaced_parameters_are_refused_until_quantised_again(change):
             m(x)
         assert not torch.equal(m.quantize_linears()(x), a)
         assert torch.equal(m(x), m(x))
+
+
+def test_optimizer_steps_replayed_from_the_callers_own_graph_are_seen():
+    import unet_amd
+    m, x = quantised_model()
+    opt = unet_amd.FusedAdamW(m.parameters(), lr=1e-2, capturable=True)
+    for i, p in enumerate(m.parameters()):
+        p.grad = make(tuple(p.shape), i, F32, 0.1).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    with torch.no_grad():
+        b = m.quantize_linears()(x)
+        assert torch.equal(m(x), b)
+        for _ in range(3):
+            graph.replay()
+            with pytest.raises(RuntimeError, match="quantize_linears"):
+                m(x)
+            c = m.quantize_linears()(x)
+            assert not torch.equal(b, c)
+            b = c
+        # a loaded optimizer state puts its step count back: still seen
+        sd = opt.state_dict()
+        graph.replay()
+        opt.load_state_dict(sd)
+        with pytest.raises(RuntimeError, match="quantize_linears"):
+            m(x)

@@ -31,3 +31,27 @@ def norm_fwd(x=P, ldx=96, f=P, ldf=96, keep=None, rps=0, qw=None, qb=None, pw=No
 def test_norm_forward_with_two_eps_refuses(kw, match):
     with pytest.raises(ValueError, match=match):
         _lib.call("unetk_gated_norm_fwd_eps", *norm_fwd(**kw))
+
+
+def test_steps_that_a_device_counter_took_are_counted():
+    """A step captured by the caller is replayed without Python: its count is the device's (a host tensor stands for it here).
+    It only ever grows, also where a loaded state puts the device's back."""
+    import unet_amd
+    from unet_amd.optim import steps_taken
+    a = torch.nn.Parameter(torch.zeros(3))
+    opt = unet_amd.FusedAdamW([a], lr=1e-3, capturable=True)
+    opt.step()      # (no gradient is there: nothing is launched)
+    hyper = torch.tensor([5.0, 1e-3, 0.0, 0.9, 0.999], dtype=torch.float64)
+    opt._hyper[0] = [hyper, None, (1e-3, 1e-2, 0.9, 0.999)]
+    opt._steps.append(hyper)
+    before = steps_taken(a)
+    hyper[0] += 2
+    assert steps_taken(a) == before + 2
+    seen = {before + 2}
+    for _ in range(3):      # steps, then back to an earlier state
+        hyper[0] += 1
+        assert steps_taken(a) not in seen
+        seen.add(steps_taken(a))
+        opt.load_state_dict({"state": {}, "param_groups": opt.state_dict()["param_groups"]})
+        assert hyper[0] == 0 and steps_taken(a) not in seen
+        seen.add(steps_taken(a))

@@ -45,8 +45,10 @@ class GraphedTrainStep:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
+        counters = list(optimizer._steps[1:])
         with torch.cuda.graph(self.graph, capture_error_mode="relaxed"):
             self.loss, parts = self._eager()
+        optimizer._steps[1:] = counters      # (this step's replays are counted here, without reading the device)
         self._parts_src = parts._pending if isinstance(parts, _LossParts) else None
         self._parts = parts
 

@@ -92,10 +92,25 @@ def clip_grad_norm_(parameters: Iterable[torch.Tensor], max_norm: float, norm_ty
     return out[0]
 
 
-def steps_taken(p) -> int:
-    """How many steps FusedAdamW optimizers have taken over this parameter (its kernel writes past autograd's version
-    counter): for what is derived from a parameter and kept beside it."""
-    return sum(n[0] for n in getattr(p, "_unetk_steps", ()))
+def steps_taken(p, read=None) -> int:
+    """A count that grows with every step that FusedAdamW optimizers take over this parameter (their kernel writes past
+    autograd's version counter): for what is derived from a parameter and kept beside it.  Where a step was captured into
+    a graph of the caller's, its replays are counted on the device only: this reads them there, waiting for the current
+    stream (read: a dict that keeps what was read, for a loop over parameters)."""
+    total = 0
+    for n in getattr(p, "_unetk_steps", ()):
+        total += n[0]
+        for hyper in n[1:]:
+            taken = None if read is None else read.get(id(hyper))
+            if taken is None:
+                if hyper.is_cuda and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("steps of a FusedAdamW captured into a graph are counted on the device, which cannot be "
+                                       "read while another graph is captured")
+                taken = int(hyper[0].item())
+                if read is not None:
+                    read[id(hyper)] = taken
+            total += taken
+    return total
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -112,7 +127,9 @@ class FusedAdamW(torch.optim.Optimizer):
         changed by a scheduler reaches the device through ``sync_hyper()``."""
         if lr < 0 or eps < 0 or not (0 <= betas[0] < 1) or not (0 <= betas[1] < 1) or weight_decay < 0:
             raise ValueError("invalid AdamW hyper-parameter")
-        self._steps = [0]       # steps taken, replays of a captured one among them: shared with the parameters
+        # Shared with the parameters, see steps_taken: the steps that Python saw, GraphedTrainStep's replays among them, and
+        # behind it the device counters (_hyper) of steps that were captured into other graphs.
+        self._steps = [0]
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None
@@ -154,6 +171,12 @@ class FusedAdamW(torch.optim.Optimizer):
                 hit[0][1:].copy_(torch.tensor(now, dtype=torch.float64), non_blocking=False)
                 hit[2] = now
 
+    def _keep_count(self):
+        """To be called before device counters are set to something else: what they counted moves to the host's count, and
+        one more, so that steps_taken only ever grows."""
+        for hyper in self._steps[1:]:
+            self._steps[0] += int(hyper[0].item()) + 1
+
     # ------------------------------------------------------------------ checkpoints
     def _pull_device_steps(self):
         """Capturable mode: graph replays advance only the device counter; bring the host-side ``step`` entries
@@ -175,6 +198,7 @@ class FusedAdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         self._fast.clear()
+        self._keep_count()
         for gi, group in enumerate(self.param_groups):
             b1, b2 = group["betas"]
             for p in group["params"]:
@@ -209,6 +233,7 @@ class FusedAdamW(torch.optim.Optimizer):
         """Puts the optimizer state back in place (same tensors, old contents; state that did not exist at the
         snapshot returns to zero)."""
         states, steps = snap
+        self._keep_count()
         for group in self.param_groups:
             for p in group["params"]:
                 st = self.state.get(p)
@@ -298,6 +323,8 @@ class FusedAdamW(torch.optim.Optimizer):
                 # (the host-side counters above only count the calls made outside graph replays; the device
                 # counter is the truth: device_step_count())
                 hyper, dyn, _ = self._hyper_for(gi, group, tl.device)
+                if torch.cuda.is_current_stream_capturing() and not any(h is hyper for h in self._steps[1:]):
+                    self._steps.append(hyper)
                 call("unetk_adamw_step_device", ptr(pp), ptr(gp), ptr(mp), ptr(vp), ptr(tl.sizes), ptr(tl.chunks),
                      tl.nchunks, ptr(hyper), ptr(dyn), float(group["eps"]), ptr(coef), 1, float(b1), float(b2), stream())
                 continue

@@ -197,8 +197,10 @@ class SwinUNet(nn.Module):
         quantised now and kept beside the parameters, their inputs on the way (ops.mx_linear).  Eval mode only: training
         steps use the parameters themselves.  A forward pass in eval mode raises once a quantised parameter has been
         changed, moved or replaced; call this again (or dequantize_linears()) after that.  (Seen are changes that count in
-        autograd's version counter, FusedAdamW's steps, replayed ones too, and another parameter or module in the place of
-        one that was there; not writes through ``parameter.data``.)  Returns self."""
+        autograd's version counter, FusedAdamW's steps, and another parameter or module in the place of one that was there;
+        not writes through ``parameter.data``.  Replays of a captured step count too: GraphedTrainStep's on the host; for a
+        graph of the caller's own each forward pass reads the optimizer's device counter, which waits for the stream and
+        is refused in a capture.)  Returns self."""
         names = []
         for li, layer in enumerate(self.layers):
             for bi in range(len(layer.blocks)):
@@ -216,7 +218,8 @@ class SwinUNet(nn.Module):
         if not all(w.is_cuda for w in weights):
             raise RuntimeError("quantize_linears: move the model to the GPU first")
         self._mx_links = list(links.values())
-        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), (w._version, steps_taken(w))) for w in weights]
+        read = {}
+        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), (w._version, steps_taken(w, read))) for w in weights]
         return self
 
     def dequantize_linears(self):
@@ -305,8 +308,9 @@ class _Ctx:
         if held is not None and not training:
             self.mx = {}
             changed = any(table.get(part) is not was for table, part, was in model._mx_links)
+            read = {}
             for w, q, at, version in held:
-                if changed or w.data_ptr() != at or (w._version, steps_taken(w)) != version:
+                if changed or w.data_ptr() != at or (w._version, steps_taken(w, read)) != version:
                     raise RuntimeError("a SwinUNet parameter was changed, moved or replaced after quantize_linears(): call it "
                                        "again, or dequantize_linears()")
                 self.mx[at] = q
