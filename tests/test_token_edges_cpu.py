@@ -55,3 +55,17 @@ def test_steps_that_a_device_counter_took_are_counted():
         opt.load_state_dict({"state": {}, "param_groups": opt.state_dict()["param_groups"]})
         assert hyper[0] == 0 and steps_taken(a) not in seen
         seen.add(steps_taken(a))
+
+
+def test_broadcast_parameters_count_as_changed(monkeypatch):
+    """The broadcast writes past autograd's version counter; what is derived from a parameter and kept beside it (4-bit
+    weights) goes by that counter."""
+    from unet_amd import dist as udist
+    m = torch.nn.Linear(3, 2)
+    monkeypatch.setattr(udist.dist, "is_initialized", lambda: True)
+    monkeypatch.setattr(udist.dist, "get_world_size", lambda *a: 2)
+    monkeypatch.setattr(udist.dist, "broadcast", lambda t, src: t.data.fill_(7.0))
+    before = [p._version for p in m.parameters()]
+    udist.broadcast_parameters(m)
+    assert all((p == 7.0).all() for p in m.parameters())
+    assert all(p._version != v for p, v in zip(m.parameters(), before))

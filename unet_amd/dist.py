@@ -242,3 +242,6 @@ def broadcast_parameters(module: torch.nn.Module, src: int = 0):
         return
     for t in list(module.parameters()) + list(module.buffers()):
         dist.broadcast(t.data, src)
+        # (written past autograd's version counter, by which what is derived from a parameter - 4-bit weights - goes)
+        if not t.is_inference():      # (which has none)
+            torch.autograd.graph.increment_version(t)
