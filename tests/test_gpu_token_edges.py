@@ -346,3 +346,31 @@ def test_optimizer_steps_replayed_from_the_callers_own_graph_are_seen():
         opt.load_state_dict(sd)
         with pytest.raises(RuntimeError, match="quantize_linears"):
             m(x)
+
+
+def test_a_captured_4_bit_prediction_follows_the_next_quantisation():
+    """The 4-bit weights stay where a captured forward pass reads them."""
+    m, x = quantised_model()
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                m(x)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, capture_error_mode="relaxed"):
+            out = m(x)
+        for k in range(4):
+            want = m(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), k
+            for layer in m.layers:
+                for blk in layer.blocks:
+                    blk.mlp[3].weight.mul_(1.25)
+            if k == 2:      # (back and again: still the same memory)
+                m.dequantize_linears()
+                torch.cuda.synchronize()
+            m.quantize_linears()

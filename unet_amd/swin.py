@@ -176,7 +176,7 @@ class SwinUNet(nn.Module):
         self.drop_path_override: Optional[List] = None
         # data-parallel hook, see unet_amd.dist.GradReducer
         self.grad_sink = None
-        self._mx_linears = self._mx_links = None         # quantize_linears()
+        self._mx_linears = self._mx_links = self._mx_kept = None         # quantize_linears()
 
     def _init_weights(self, m):
         # reference swin_unet_model.py:616-630 (ConvTranspose2d is not a Conv2d: keeps its default init)
@@ -200,7 +200,8 @@ class SwinUNet(nn.Module):
         autograd's version counter, FusedAdamW's steps, and another parameter or module in the place of one that was there;
         not writes through ``parameter.data``.  Replays of a captured step count too: GraphedTrainStep's on the host; for a
         graph of the caller's own each forward pass reads the optimizer's device counter, which waits for the stream and
-        is refused in a capture.)  Returns self."""
+        is refused in a capture.)  A captured forward pass reads the 4-bit weights where they lie: replays take those of the
+        last call of this.  Returns self."""
         names = []
         for li, layer in enumerate(self.layers):
             for bi in range(len(layer.blocks)):
@@ -217,13 +218,22 @@ class SwinUNet(nn.Module):
             weights.append(at)
         if not all(w.is_cuda for w in weights):
             raise RuntimeError("quantize_linears: move the model to the GPU first")
-        self._mx_links = list(links.values())
         read = {}
-        self._mx_linears = [(w, ops.mx_quantize(w.detach()), w.data_ptr(), (w._version, steps_taken(w, read))) for w in weights]
+        marks = [(w.data_ptr(), (w._version, steps_taken(w, read))) for w in weights]
+        quantised = [ops.mx_quantize(w.detach()) for w in weights]
+        # into the memory of the last call, which captured forward passes read
+        kept = self._mx_kept or [None] * len(weights)
+        for i, (q, old) in enumerate(zip(quantised, kept)):
+            if old is not None and (old.shape, old.index) == (q.shape, q.index):
+                old.data.copy_(q.data)
+                quantised[i] = old
+        self._mx_kept, self._mx_links = quantised, list(links.values())
+        self._mx_linears = [(w, q) + mark for w, q, mark in zip(weights, quantised, marks)]
         return self
 
     def dequantize_linears(self):
-        """Back to the parameters themselves in eval mode.  Returns self."""
+        """Back to the parameters themselves in eval mode (the 4-bit weights stay in memory for forward passes that were
+        captured with them).  Returns self."""
         self._mx_linears = self._mx_links = None
         return self
 
