@@ -374,3 +374,28 @@ def test_a_captured_4_bit_prediction_follows_the_next_quantisation():
                 m.dequantize_linears()
                 torch.cuda.synchronize()
             m.quantize_linears()
+
+
+def test_a_captured_step_takes_an_optimizer_that_wraps_the_fused_one():
+    import unet_amd
+    from unet_amd.graph import GraphedTrainStep
+    x, y, _ = W.synthetic_batch(1, 4, 64, 64, seed=42)
+    m, _, cfg = swin(F32)
+    m.train()
+    m.drop_path_override = [[None, None]] * sum(cfg["depths"])
+    inner = unet_amd.FusedAdamW(m.parameters(), lr=1e-3, capturable=True)
+
+    class Wrapper:
+        capturable = True
+        zero_grad, step, sync_hyper = inner.zero_grad, inner.step, inner.sync_hyper
+        snapshot, restore = inner.snapshot, inner.restore
+    loss = lambda out, label: ((out - F.interpolate(label, out.shape[-2:])) ** 2).mean()
+    step = GraphedTrainStep(m, loss, Wrapper(), x.cuda(), y.cuda(), warmup=2)
+    with torch.no_grad():
+        a = m.eval().quantize_linears()(x.cuda())
+        for _ in range(2):
+            step(x.cuda(), y.cuda())
+            with pytest.raises(RuntimeError, match="quantize_linears"):
+                m(x.cuda())
+        assert not torch.equal(m.quantize_linears()(x.cuda()), a)
+    assert inner.device_step_count() == 2

@@ -45,10 +45,12 @@ class GraphedTrainStep:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self.graph = torch.cuda.CUDAGraph()
-        counters = list(optimizer._steps[1:])
+        self._steps = getattr(optimizer, "_steps", None)      # (none: an optimizer that wraps the fused one)
+        counters = None if self._steps is None else self._steps[1:]
         with torch.cuda.graph(self.graph, capture_error_mode="relaxed"):
             self.loss, parts = self._eager()
-        optimizer._steps[1:] = counters      # (this step's replays are counted here, without reading the device)
+        if counters is not None:      # (this step's replays are counted here, without reading the device)
+            self._steps[1:] = counters
         self._parts_src = parts._pending if isinstance(parts, _LossParts) else None
         self._parts = parts
 
@@ -75,7 +77,8 @@ class GraphedTrainStep:
         if self.w is not None and w is not None and w.data_ptr() != self.w.data_ptr():
             self.w.copy_(w, non_blocking=True)
         self.optimizer.sync_hyper()
-        self.optimizer._steps[0] += 1
+        if self._steps is not None:
+            self._steps[0] += 1
         self.graph.replay()
         parts = _LossParts(*self._parts_src) if self._parts_src is not None else self._parts
         return self.loss, parts
