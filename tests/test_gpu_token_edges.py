@@ -399,3 +399,35 @@ def test_a_captured_step_takes_an_optimizer_that_wraps_the_fused_one():
                 m(x.cuda())
         assert not torch.equal(m.quantize_linears()(x.cuda()), a)
     assert inner.device_step_count() == 2
+
+
+def test_weights_are_quantised_again_in_and_out_of_inference_mode():
+    m, x = quantised_model()
+    with torch.inference_mode():
+        want = m(x).clone()
+        m.quantize_linears()
+    with torch.no_grad():
+        assert torch.equal(m(x), want)
+    m.dequantize_linears()
+    fresh, _ = quantised_model()
+    fresh.dequantize_linears()
+    fresh._mx_kept = None
+    with torch.inference_mode():
+        fresh.quantize_linears()      # (memory that was made in inference mode)
+    fresh.quantize_linears()
+    with torch.no_grad():
+        assert torch.equal(fresh(x), want)
+
+
+def test_quantisation_into_memory_that_is_there():
+    from unet_amd import ops
+    for dt in (F32, BF):
+        a, b = make((70, 200), 1, dt).cuda(), make((70, 200), 2, dt).cuda()
+        q, want = ops.mx_quantize(a), ops.mx_quantize(b)
+        at = q.data.data_ptr()
+        assert ops.mx_quantize(b, out=q) is q and q.data.data_ptr() == at and torch.equal(q.data, want.data)
+        for bad in (a[:, :199], a[:64], a.view(7, 10, 200)):
+            with pytest.raises(ValueError, match="out"):
+                ops.mx_quantize(bad, out=q)
+        with pytest.raises(TypeError, match="out"):
+            ops.mx_quantize(a, out=b)

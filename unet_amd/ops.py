@@ -1143,27 +1143,33 @@ class MxTensor:
         return f"MxTensor(shape={tuple(self.shape)}, device={self.device})"
 
 
-def mx_quantize(x) -> MxTensor:
+def mx_quantize(x, out: Optional[MxTensor] = None) -> MxTensor:
     """x (..., K), float32 or bfloat16 with equally spaced rows, in 4 bits: per block of 32 along K the scale
     2^(floor(log2 max) - 2) and the elements rounded half to even to 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (larger ones:
     6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros.  It has no
-    gradient, and refuses an x that wants one."""
+    gradient, and refuses an x that wants one.  out: an MxTensor of x's shape to write to (and return)."""
     rows, ld = _token_rows(x, "x")
     _no_gradient("mx_quantize", x)
     code, K, dev = dtype_code(x.dtype), x.shape[-1], x.get_device()
     if K < 1:
         raise ValueError("mx_quantize: no elements to scale (K = 0)")
+    if out is not None:
+        if not isinstance(out, MxTensor):
+            raise TypeError(f"mx_quantize: out is an MxTensor, got {type(out).__name__}")
+        if out.shape != x.shape or out.index != dev:
+            raise ValueError(f"mx_quantize: out {tuple(out.shape)} on {out.device} for x {tuple(x.shape)} on {x.device}")
     if dev != _raw_device():
         with torch.cuda.device(dev):
-            return mx_quantize(x)
+            return mx_quantize(x, out)
     nc = _lib.load().unetk_mx_codes_bytes(rows, K) if rows else 0
     if rows and not nc:
         raise ValueError(f"mx_quantize: a {rows} x {K} matrix is too large")
-    data = torch.empty(nc + nc // 16, dtype=torch.uint8, device=x.device)
+    if out is None:
+        out = MxTensor(torch.empty(nc + nc // 16, dtype=torch.uint8, device=x.device), nc, x.shape)
     if rows:
-        at = data.data_ptr()
+        at = out.data.data_ptr()
         call("unetk_mx_quantize", x.data_ptr(), ld, rows, K, code, at, at + nc, stream())
-    return MxTensor(data, nc, x.shape)
+    return out
 
 
 def mx_dequantize(q: MxTensor, dtype=torch.bfloat16) -> torch.Tensor:

@@ -220,13 +220,10 @@ class SwinUNet(nn.Module):
             raise RuntimeError("quantize_linears: move the model to the GPU first")
         read = {}
         marks = [(w.data_ptr(), (w._version, steps_taken(w, read))) for w in weights]
-        quantised = [ops.mx_quantize(w.detach()) for w in weights]
         # into the memory of the last call, which captured forward passes read
         kept = self._mx_kept or [None] * len(weights)
-        for i, (q, old) in enumerate(zip(quantised, kept)):
-            if old is not None and (old.shape, old.index) == (q.shape, q.index):
-                old.data.copy_(q.data)
-                quantised[i] = old
+        quantised = [ops.mx_quantize(w.detach(), q if q is not None and (q.shape, q.index) == (w.shape, w.get_device()) else None)
+                     for w, q in zip(weights, kept)]
         self._mx_kept, self._mx_links = quantised, list(links.values())
         self._mx_linears = [(w, q) + mark for w, q, mark in zip(weights, quantised, marks)]
         return self
