@@ -431,3 +431,47 @@ def test_quantisation_into_memory_that_is_there():
                 ops.mx_quantize(bad, out=q)
         with pytest.raises(TypeError, match="out"):
             ops.mx_quantize(a, out=b)
+
+
+def test_a_gradient_sink_gets_the_gradients_of_every_parameter():
+    m, _, cfg = swin(BF, post_norm=True, layer_scale=0.5)
+    x = W.synthetic_batch(2, 4, 64, 64, seed=42)[0].cuda()
+    m.train()
+    m.drop_path_override = [[None, None]] * sum(cfg["depths"])
+    m(x).square().mean().backward()
+    plain = {k: p.grad.clone() for k, p in m.named_parameters()}
+    m.zero_grad(set_to_none=True)
+    seen = {}
+
+    def sink(name, t):
+        seen[name] = t.clone()      # (on the stream that made it)
+        return t
+    m.grad_sink = sink
+    m(x).square().mean().backward()
+    torch.cuda.synchronize()
+    for k in plain:
+        assert torch.equal(seen[k], plain[k]), k
+
+
+def test_4_bit_prediction_in_float32():
+    """With a float32 compute type the pass quantises the same way; the two types' outputs differ by the bfloat16 pass's
+    roundings and by the 4 bits that these turn over, and by far less than a wrong product would make of it."""
+    m, x = quantised_model(F32)
+    with torch.no_grad():
+        q = m(x)
+        assert q.dtype == F32 and torch.isfinite(q).all() and torch.equal(m(x), q)
+        assert not torch.equal(m.dequantize_linears()(x), q)
+
+
+def test_a_copied_model_is_refused_until_quantised_by_itself():
+    import copy
+    m, x = quantised_model()
+    with torch.no_grad():
+        a = m(x)
+        other = copy.deepcopy(m)
+        with pytest.raises(RuntimeError, match="quantize_linears"):
+            other(x)
+        other.layers[0].blocks[0].mlp[0].weight.mul_(1.5)
+        assert not torch.equal(other.quantize_linears()(x), a)
+        assert torch.equal(m(x), a)      # (nothing is shared between the two)
+        assert torch.equal(m.quantize_linears()(x), a)
