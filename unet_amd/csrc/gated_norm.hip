@@ -13,10 +13,13 @@
 // unrounded r (which is in registers), and the backward pass forms r again from x and f for the same reason: it reads
 // as many bytes as with a stored r.
 //
-// Measured (MI355X; a large copy reaches 5.0 TB/s here), bf16 unless noted: forward 262144 x 96 43.2 us (4.7 TB/s),
-// 65536 x 192 27.2 us (3.7), 8192 x 4096 RMS 57.0 us (4.7); backward 65536 x 192 30.3 us (5.0 TB/s), 8192 x 4096 77.8 us (5.2),
-// each followed by 5...8 us of column sums; 5003 x 1001 fp32 19.5, 26.6 and 6 us (4.1 and 4.5 TB/s); 64 x 768 forward 5.6 us,
-// which is a launch and one pass through the loads.
+// Measured (MI355X; a large copy reaches 5.0 TB/s here; the kernel alone, operands out of the caches), bf16 unless noted:
+// forward 262144 x 96 43.7 us (4.6 TB/s), 65536 x 192 27.5 us (3.7), 8192 x 4096 RMS 52.0 us (5.2); backward 65536 x 192 30.7 us
+// (4.9 TB/s), 8192 x 4096 72.8 us (5.5), each followed by 5...8 us of column sums; 5003 x 1001 fp32 19.0, 26.4 and 6.6 us (4.2
+// and 4.6 TB/s); 64 x 768 forward 7.3 us (5.4 with its operands in the caches), which is a launch and one pass through the loads.
+//
+// Infinities and NaN stay in their row, and in the column sums of their channels.  (With a bias behind the branch dgate is two
+// sums' combination: where both are infinite it may be NaN for an infinity of the definition.)
 #include "unaligned.h"
 
 namespace {
@@ -40,7 +43,7 @@ struct NormArgs {
 
 // The elements of a row that one of its G lanes holds: N = NV 16-byte vectors, at whatever address the row begins.
 // WHOLE: C is a multiple of the vector's elements; else the lanes take single elements side by side (20000 x 1001 bf16
-// forward: 44.4 us so, 59.2 with vectors off their alignment; 5003 x 1001 fp32: 17.2 and 22.0).
+// forward: 44.4 us so, 59.2 with vectors off their alignment; 5003 x 1001 fp32: 17.2 and 22.0; operands cached).
 template <typename T, int G, int NV, bool WHOLE> struct Lane {
   static constexpr int E = Vec16<T>::N, N = NV * E;
   static constexpr bool SINGLE = !WHOLE;

@@ -93,8 +93,8 @@ __device__ __forceinline__ void load_block(const T* row, int k0, int K, bool the
     x.v[j] = __builtin_bit_cast(u32x4, load_part<WHOLE>(row + k0 + j * E, there ? K - (k0 + j * E) : 0));
 }
 
-// One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x: 65536 x 768 bf16 28.7 us (127 MB,
-// 4.4 TB/s), 8192 x 8192 47 us (170 MB, 3.6 TB/s).  (One workgroup of four waves a unit: with a wave a unit, four fragments in
+// One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x: 65536 x 768 bf16 28.5 us (127 MB,
+// 4.5 TB/s), 8192 x 8192 40.1 us (170 MB, 4.2 TB/s), operands out of the caches.  (One workgroup of four waves a unit: with a wave a unit, four fragments in
 // turn, a small matrix has too few waves to hide its loads.)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t rows, int K,
@@ -123,7 +123,7 @@ __device__ __forceinline__ float mx_value(uint32_t code, uint32_t scale) {
 }
 
 // One workgroup a unit; a lane makes 8 consecutive values, 16 lanes the 128 of a row: runs of 256 bytes (bf16) a row.  Bound
-// by the write of the values: 65536 x 768 to bf16 22.8 us (127 MB, 5.6 TB/s: much of the codes still lies in the last cache).
+// by the write of the values: 65536 x 768 to bf16 22.5 us (127 MB, 5.6 TB/s: much of the codes still lies in the last cache).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                             uint32_t rows, int K, uint32_t kt, T* __restrict__ out, int64_t ldo) {
@@ -371,8 +371,9 @@ template <typename F> __device__ __forceinline__ void with_epilogue(const MxArgs
 
 // ---- few tiles: the W waves of a workgroup share the steps of K of one tile of SIDE x SIDE outputs and add their sums
 // through LDS in a fixed tree.  SRC: the activations' own type, quantised by each wave for its steps, or void: packed.
-// A step's fragments are fetched one step ahead.  Bound by latency: 1 x 4096 -> 4096 5.2 us replayed from a graph (8.9 MB of
-// weights, 1.8 us at 5 TB/s), 1037 x 2072 -> 1511 fp32 9 us.
+// A step's fragments are fetched one step ahead.  Bound by latency: 1 x 4096 -> 4096, quantising on the way, 7.6 us with the
+// weights out of the caches (8.9 MB, 1.8 us at 5 TB/s), 6.1 with them in; 1037 x 2072 -> 1511 fp32, quantised before, 13.8 and
+// 11.6.  (A launch among others replayed from a graph takes about 1 us less than alone: 5.2 and 10.8, cached.)
 
 // one 16 x 16 tile (16x16x128: lane l holds row l % 16, k block l / 16), its fragments gathered from the units by blocks
 struct Tile16 {
@@ -556,9 +557,10 @@ __global__ __launch_bounds__(1024) void mx_split_kernel(MxArgs a) {
 // waves take every W-th group of 64 columns.  The weights' fragments come straight from the caches into
 // a ring of registers, a group ahead; the rows' are read from LDS a step at a time.  Bound by the write of the output (a
 // store instruction whose lanes lie in many rows holds the CU's address path for some 100 cycles) and the arithmetic on it.
-// 262144 x 96 -> 384 with GELU 75 us (252 MB, 3.4 TB/s, a floor of 50; 51 without GELU and with 288 columns); 16384 x 384 -> 1152
-// 15.1 us (50 MB, 3.3 TB/s).  With stores of 32 bytes in each of 32 rows the first took 90 us, 17 of them behind the
-// kernel's end, and 61 where the output stayed in the last cache; stores past the caches 204.
+// 262144 x 96 -> 384 with GELU 70.3 us (252 MB, 3.6 TB/s, a floor of 50), 62.9 with the operands cached; 16384 x 384 -> 1152 16.9
+// us (50 MB, 3.0 TB/s), 15.8 cached.  (Stores of 32 bytes in each of 32 rows took 18 us more on the first, 17 of them behind
+// the kernel's end, and nothing more where the output stayed in the last cache; stores past the caches 130 more.  With a residual
+// they are still taken: 262144 x 96 -> 96 31.1 us, 262144 x 384 -> 96 80.4, replayed from a graph; floors of 30 and 60.)
 template <typename T, typename SRC, int KS>
 __global__ __launch_bounds__(512, KS <= 2 ? 4 : KS <= 4 ? 3 : 2) void mx_rows_kernel(MxArgs a) {
   constexpr bool RAW = !std::is_void<SRC>::value;
@@ -664,7 +666,9 @@ __global__ __launch_bounds__(512, KS <= 2 ? 4 : KS <= 4 ? 3 : 2) void mx_rows_ke
 // ---- large products: 256 x 256 outputs a workgroup, 128 x 128 a wave, so that a byte read from LDS meets 128 others.
 // Four LDS stages of a step (128 k) each, filled by LDS-DMA: while step s multiplies from registers, the fragments of step
 // s + 1 are read from their stage between the multiplications, stage s + 2 is landing and s + 3 is requested.
-// 8192^3: 250...290 us (3.8...4.4 PFLOP/s; 10 are nominal, 8.4 what the instruction reaches from registers alone with such data).
+// 8192^3: 263...275 us with pauses between the launches, 260...320 one behind the other (3.4...4.2 PFLOP/s; 10 are nominal, 8.4 what
+// the instruction reaches from registers alone with such data); fp32 results 409, bf16 with a residual 303 (stored straight
+// from the registers, the former with 48 of them spilled in the epilogue), replayed from a graph, 248 without.
 // The chip lowers its clock to 1.87 GHz during it and the matrix pipe is busy half of the cycles.
 // LDS-DMA of 16 bytes a lane as an instruction of its own.  Through the builtin the compiler follows which transfers may
 // still be filling which array, loses track at the loop's end and waits for all of them there, the newest included; here
@@ -849,7 +853,7 @@ int check_mx(const char* who, int64_t rows, int64_t K, int dtype) {
 }
 
 // Which kernel takes an M x N x K product: by sizes alone, so that activations quantised beforehand give the same bits.
-// Times in us, bf16, replayed from a graph.
+// Times in us, bf16, replayed from a graph on the same operands (as all figures of the rules below).
 //   rows against quantisation and split (short K): 1024 x 192 -> 768 5.8 and 5.8, 2048 rows 6.0 and 6.6; x 384 -> 1152: 1024 rows
 //   7.2 and 6.8, 2048 7.6 and 8.1; x 768 -> 2304: 2048 rows 14.5 and 13.3, 4096 19.0 and 21.7: from 512 rows a step of K on;
 //   large against split: 64 tiles (2048 x 2048) 28.2 and 24.3 with K = 4096, 14.5 and 9.6 with 1024; 96 tiles (2048 x 3000) 28.9
@@ -865,9 +869,10 @@ Plan plan_of(int64_t M, int64_t K, int64_t N) {
 // the split kernel's tile, 16 or 32 a side: 32 x 4096 -> 4096 4.4 and 4.9 us, 64 x 4096 -> 4096 5.6 and 5.2, 256 x 1024 -> 1024 3.7
 // both, 512 x 4096 -> 512 5.6 and 5.2.  (64 a side: 1024 x 1024 -> 1024 7.5 against 4.7 with 32, 2048 x 4096 -> 2048 22.6 against 24.3.)
 bool small_tiles(int64_t M, int64_t N) { return M * N < 1 << 18; }
-// Activations quantised inside the product, by every tile of columns again, or by a launch of their own: bf16 4 x 4096 -> 4096
-// 5.7 and 6.1 us, 8 x 4096 -> 4096 6.3 and 6.1, 16 x 2048 -> 2048 5.2 and 5.7, 16 x 4096 -> 4096 7.8 and 6.2; fp32 1 x 4096 -> 4096 6.3
-// both, 16 x 1024 -> 1024 5.0 and 5.4, 4 x 4096 -> 4096 7.1 and 6.3.
+// Activations quantised inside the product, by every tile of columns again, or by a launch of their own: bf16 1 x 4096 -> 4096
+// 5.4 and 6.5 us, 4 x 4096 -> 4096 5.6 and 6.7, 8 x 4096 -> 4096 6.1 and 6.7, 16 x 2048 -> 2048 5.4 and 5.9, 16 x 4096 -> 4096 7.8 and 6.8;
+// fp32 1 x 4096 -> 4096 6.3 and 6.6, 4 x 4096 -> 4096 7.0 and 6.7.  The rule does not see N: with many columns the launch of its own
+// would win (4 x 4096 -> 16384 15.8 and 12.5, 8 x 4096 -> 65536 45.6 and 25.7).
 bool quantised_inside(int64_t M, int64_t K, int64_t N, int dtype) {
   if (K % (dtype == UNETK_BF16 ? 8 : 4) != 0) return false;
   const Plan p = plan_of(M, K, N);
