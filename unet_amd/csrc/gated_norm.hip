@@ -305,9 +305,19 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
   const uint32_t step = gridDim.x * RPB;
   if (blockIdx.x * RPB < a.M) fetch(blockIdx.x * RPB);
   for (uint32_t row0 = blockIdx.x * RPB; row0 < a.M; row0 += step) {
-    const bool live = RPB == 1 || row0 + rg < a.M;
+    const bool live = row0 + rg < a.M;
     const uint32_t row = live ? row0 + rg : row0;
-    const typename L::Raw xr = nx.x, fr = nx.f, dr = nx.dr, dn = nx.dn;
+    const typename L::Raw xr = nx.x, dr = nx.dr, dn = nx.dn;
+    typename L::Raw fr = nx.f;
+    if (RPB > 1) {      // (lanes past the last row hold its values again: zero times an infinite one would be NaN)
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        u32x4 v = __builtin_bit_cast(u32x4, fr.v[k]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live ? v[e] : 0u;
+        fr.v[k] = __builtin_bit_cast(Vec16<T>, v);
+      }
+    }
     const f32x4 st = nx.st;
     const float keep = nx.keep;
     if (row0 + step < a.M) fetch(row0 + step);
@@ -340,8 +350,7 @@ __global__ __launch_bounds__(threads_of(G)) void gated_norm_bwd_kernel(NormArgs 
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      // (lanes past the last row hold its values again: zero times an infinite one would be NaN)
-      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f, fh = live ? norm_hat(L::at(fr, i), fm, fs) : 0.f;
+      const float u = (live && ln.has(i)) ? keep * g[i] : 0.f, fh = norm_hat(L::at(fr, i), fm, fs);
       acc[2][i] += u * fh;
       acc[3][i] += u;
       o[i] = u * prm(0, i);

@@ -1116,12 +1116,10 @@ def gated_norm_bwd(dr, dn, x, f, stats, gate=None, keep=None, res_scale=1.0, pos
     return GatedNormGrads(dx, df, dg, dqw, dqb, dpw, dpb)
 
 
-def _no_gradient(what, *tensors):
-    """Refuses inputs (None: not given) that want a gradient: autograd does not see the call, and theirs would be lost."""
+def _no_gradient(what):
+    """Refuses a call one of whose inputs wants a gradient: autograd does not see it, and the gradient would be lost."""
     if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach its inputs")
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or detach its inputs")
 
 
 class MxTensor:
@@ -1149,7 +1147,8 @@ def mx_quantize(x, out: Optional[MxTensor] = None) -> MxTensor:
     6).  A block with a NaN or an infinity becomes NaN as a whole.  A short last block is filled with zeros.  It has no
     gradient, and refuses an x that wants one.  out: an MxTensor of x's shape to write to (and return)."""
     rows, ld = _token_rows(x, "x")
-    _no_gradient("mx_quantize", x)
+    if x.requires_grad:
+        _no_gradient("mx_quantize")
     code, K, dev = dtype_code(x.dtype), x.shape[-1], x.get_device()
     if K < 1:
         raise ValueError("mx_quantize: no elements to scale (K = 0)")
@@ -1232,7 +1231,9 @@ def mx_linear(x, w: MxTensor, bias=None, act=0, resid=None, out=None, dtype=None
             if resid is not None and not (resid.data_ptr() == to and ldr == ldo) and \
                     not _apart(resid.data_ptr(), N * e, to, N * e, rows, ldr * e, ldo * e):
                 raise ValueError("mx_linear: out shares memory with resid without being resid")
-    _no_gradient("mx_linear", None if quantised else x, bias, resid, out)
+    if (not quantised and x.requires_grad) or (bias is not None and bias.requires_grad) or \
+            (resid is not None and resid.requires_grad) or (out is not None and out.requires_grad):
+        _no_gradient("mx_linear")
     if dev != _raw_device():
         with torch.cuda.device(dev):
             return mx_linear(x, w, bias, act, resid, out, dtype)
