@@ -475,3 +475,18 @@ def test_a_copied_model_is_refused_until_quantised_by_itself():
         assert not torch.equal(other.quantize_linears()(x), a)
         assert torch.equal(m(x), a)      # (nothing is shared between the two)
         assert torch.equal(m.quantize_linears()(x), a)
+
+
+def test_blocks_added_between_two_quantisations_are_quantised():
+    from unet_amd.swin import SwinTransformerBlock
+    m, x = quantised_model()
+    n = len(m._mx_linears)
+    with torch.no_grad():
+        m(x)
+        b = m.layers[1].blocks[0]
+        m.layers[1].blocks.append(SwinTransformerBlock(b.dim, b.num_heads, b.window_size, 0, b.mlp_ratio).cuda().eval())
+        m.quantize_linears()
+        assert len(m._mx_linears) == n + 4
+        want = m(x)
+        m._mx_kept = None      # (into fresh memory)
+        assert torch.equal(m.quantize_linears()(x), want)

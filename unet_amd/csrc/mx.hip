@@ -94,8 +94,8 @@ __device__ __forceinline__ void load_block(const T* row, int k0, int K, bool the
 }
 
 // One wave: a fragment (32 rows x 64 k), each lane one block.  Bound by the read of x: 65536 x 768 bf16 28.5 us (127 MB,
-// 4.5 TB/s), 8192 x 8192 40.1 us (170 MB, 4.2 TB/s), operands out of the caches.  (One workgroup of four waves a unit: with a wave a unit, four fragments in
-// turn, a small matrix has too few waves to hide its loads.)
+// 4.5 TB/s), 8192 x 8192 40.1 us (170 MB, 4.2 TB/s), operands out of the caches.  (One workgroup of four waves a unit: with a
+// wave a unit, four fragments in turn, a small matrix has too few waves to hide its loads.)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, int64_t ldx, uint32_t rows, int K,
                                                           uint32_t kt, u32x4* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -667,8 +667,8 @@ __global__ __launch_bounds__(512, KS <= 2 ? 4 : KS <= 4 ? 3 : 2) void mx_rows_ke
 // Four LDS stages of a step (128 k) each, filled by LDS-DMA: while step s multiplies from registers, the fragments of step
 // s + 1 are read from their stage between the multiplications, stage s + 2 is landing and s + 3 is requested.
 // 8192^3: 263...275 us with pauses between the launches, 260...320 one behind the other (3.4...4.2 PFLOP/s; 10 are nominal, 8.4 what
-// the instruction reaches from registers alone with such data); fp32 results 409, bf16 with a residual 303 (stored straight
-// from the registers, the former with 48 of them spilled in the epilogue), replayed from a graph, 248 without.
+// the instruction reaches from registers alone with such data).  Replayed from a graph: 248, with a residual 303, fp32 results
+// 409 (both stored straight from the registers, the latter with 48 of them spilled in the epilogue).
 // The chip lowers its clock to 1.87 GHz during it and the matrix pipe is busy half of the cycles.
 // LDS-DMA of 16 bytes a lane as an instruction of its own.  Through the builtin the compiler follows which transfers may
 // still be filling which array, loses track at the loop's end and waits for all of them there, the newest included; here

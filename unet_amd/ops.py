@@ -1046,9 +1046,9 @@ def gated_norm_fwd(x, f, gate=None, keep=None, res_scale=1.0, post=None, pre=Non
 
     x: the residual stream, f: the branch's output, (..., C) float32 or bfloat16 with equally spaced rows (dense, or a
     channel slice).  post, pre: (weight, bias or None) of the two norms, each may be None; kind: "layer" or "rms" (without
-    the mean); eps: under both norms' roots, or a pair of them, post's and pre's.  gate: (C,) factors (layer scale); keep: one DropPath factor a sample, samples outermost.  Parameters are
-    float32.  Returns (r, n, stats): r and n dense, n None without pre; stats is what gated_norm_bwd reads (None unless
-    want_stats).  n is taken from the unrounded r."""
+    the mean); eps: under both norms' roots, or a pair of them, post's and pre's.  gate: (C,) factors (layer scale); keep:
+    one DropPath factor a sample, samples outermost.  Parameters are float32.  Returns (r, n, stats): r and n dense, n None
+    without pre; stats is what gated_norm_bwd reads (None unless want_stats).  n is taken from the unrounded r."""
     a_keep = keep
     M, C, dev, ldx, ldf, code, g, keep, rps, qw, qb, pw, pb = _gated_norm_args(x, f, gate, keep, post, pre, kind)
     post_eps, pre_eps = eps if isinstance(eps, (tuple, list)) else (eps, eps)

@@ -127,6 +127,8 @@ class DecoderBlock(nn.Module):
 
 
 class SwinUNet(nn.Module):
+    _mx_linears = _mx_links = _mx_kept = None       # quantize_linears()
+
     def __init__(self, config_dict, compute_dtype=torch.float32):
         super().__init__()
         c = config_dict
@@ -176,7 +178,6 @@ class SwinUNet(nn.Module):
         self.drop_path_override: Optional[List] = None
         # data-parallel hook, see unet_amd.dist.GradReducer
         self.grad_sink = None
-        self._mx_linears = self._mx_links = self._mx_kept = None         # quantize_linears()
 
     def _init_weights(self, m):
         # reference swin_unet_model.py:616-630 (ConvTranspose2d is not a Conv2d: keeps its default init)
@@ -213,6 +214,8 @@ class SwinUNet(nn.Module):
             at = self
             for part in name.split("."):      # where each module and parameter on the way hangs, to see it replaced
                 table = at._parameters if part in at._parameters else at._modules
+                if part not in table:
+                    raise RuntimeError(f"quantize_linears: {name} is not a parameter of the model's own")
                 at = table[part]
                 links[id(table), part] = (table, part, at)
             weights.append(at)
@@ -221,7 +224,7 @@ class SwinUNet(nn.Module):
         read = {}
         marks = [(w.data_ptr(), (w._version, steps_taken(w, read))) for w in weights]
         # into the memory of the last call, which captured forward passes read
-        kept = self._mx_kept or [None] * len(weights)
+        kept = (self._mx_kept or []) + [None] * len(weights)
         quantised = [ops.mx_quantize(w.detach(), q if q is not None and (q.shape, q.index) == (w.shape, w.get_device()) else None)
                      for w, q in zip(weights, kept)]
         self._mx_kept, self._mx_links = quantised, list(links.values())
